@@ -1,0 +1,94 @@
+/* The attention half of a decode step, and the token at its end. No counterpart on the reference's side of this library: there the
+ * cache and the attention are the engine's, the sampling the server's.
+ *
+ *     qw_kv_write()   rows of queries, keys and values: queries and keys turned by their positions, keys and values into the cache
+ *     qw_kv_read()    such rows of keys and values back out of it
+ *     qw_attn()       the queries' attention over the cache
+ *     qw_sample()     a token a row out of the vocabulary's logits
+ *
+ * Each records into a batch (qw_batch_begin) as the functions of qw_path.h do, or into a recorder on a stream of the caller's
+ * (qw_hip_stream_begin, below). Failure: false and a text in qw_hip_last_error; the batch has then failed, nothing of it is launched.
+ *
+ * The cache. Pages of `page` tokens (a power of two from 16), each with all heads of the layer; page p lies at offset + p * (bytes of a
+ * page), in it head after head, in each head units of 16 tokens. A unit holds, for D = dim values a head (tokens t, values v),
+ *     F16 (type 1), 64 D bytes:   keys [D/8][16 t][8 v], values [D/32][4][32 v][4 t]
+ *     Q8_0 (type 8), 34 D bytes:  keys [D/64][4][16 t][2][8] int8 (value 64 a + 32 b + 8 c + d at [a][c][t][b][d]), scales of the keys
+ *                                 [4][D/32][4 t], values [D/64][4][16][2][2][4 t] int8 (value 64 a + 32 b + 2 c + d at [a][.][c][b][d]), scales
+ *                                 of the values [4][D/32][4 t]; scales are binary16, one for 32 values of a token
+ * with t = 4 [first of the 4s] + [last of the 4s]. It is the order in which the matrix instructions take them. Q8_0 of 32 values x: d = max |x| / 127 rounded
+ * to binary16, codes round(x / d) (0 where d is 0); 32 values of which one is not finite are held as NaN.
+ *
+ * A step. Slot i (a conversation) has rows first[i] .. first[i + 1) of the step's `rows`, and, those included, len[i] tokens: its row j
+ * is token len[i] - n + j, n = first[i + 1] - first[i]. Token t lies in page table[i][t / page]. first, len and table are read on the device
+ * when the kernels run, so a captured sequence goes on being right as the slots grow. Rows that belong to no slot are left as they are. What the
+ * device finds there cannot be refused any more, and nothing out of bounds is touched for it: a slot whose rows do not lie in the step has
+ * none, len counts up to max_pages * page, a page number from `pages` on is no page - its tokens are not written, read back as zeros and not
+ * attended to.
+ */
+#pragma once
+#include "gpu.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+typedef struct { const qw_buf *buf; size_t offset; } qw_at;
+
+typedef struct {
+    qw_at at; /* 16-byte aligned; keep it device-only (qw_hip_buf_new_device): a shadow would be copied back after every write */
+    int type, heads, dim, page, pages; /* ggml type 1 or 8; dim 64, 128, 192 or 256 */
+} qw_kv;
+/* Bytes of such a cache; 0 if this build has none like it. */
+size_t qw_kv_bytes(int type, int heads, int dim, int page, int pages);
+
+#define QW_KV_MAX_SLOTS 256
+#define QW_KV_MAX_ROWS 65536
+typedef struct {
+    int slots, rows, max_pages;
+    qw_at first; /* uint32 [slots + 1], not decreasing */
+    qw_at len;   /* uint32 [slots] */
+    qw_at table; /* uint32 [slots][max_pages] */
+} qw_kv_step;
+
+/* Binary16 rows of some heads of dim values each, `stride` values from one row to the next (a multiple of 8; 0: heads * dim);
+ * 16-byte aligned. */
+typedef struct { qw_at at; int stride; } qw_kv_rows;
+
+/* Rotary positions: the first `dims` values of a head (even) turn in pairs, value i with i + dims / 2, or with adjacent 2 i with 2 i + 1.
+ * Pair i turns by pos[row][axis] * freq[i] radians; the first pairs[0] pairs go by axis 0, the next pairs[1] by axis 1, the others by axis 2
+ * (axes = 1: all by axis 0; pairs[2] makes up dims / 2). Angles and products in 64 bits, rounded to binary16 once. */
+typedef struct {
+    int dims, axes, pairs[3]; /* axes 1 or 3 */
+    bool adjacent;
+    qw_at freq; /* double [dims / 2] */
+    qw_at pos;  /* int32 [rows][axes] */
+} qw_rope;
+
+/* The step's rows: q turned into q_out (which may be q itself), k turned and v as it is into the cache. rope NULL: nothing turns. q_heads 0: no
+ * queries. */
+bool qw_kv_write(qw_batch *b, const qw_kv *c, const qw_kv_step *s, const qw_rope *rope, int q_heads, const qw_kv_rows *q, const qw_kv_rows *q_out, const qw_kv_rows *k,
+                 const qw_kv_rows *v);
+/* The rows' tokens out of the cache. Any range of tokens is a step: rows first[i] .. and len[i] where the range ends. */
+bool qw_kv_read(qw_batch *b, const qw_kv *c, const qw_kv_step *s, const qw_kv_rows *k, const qw_kv_rows *v);
+
+/* out[row][h] = the mean of its slot's values, weighted by softmax(scale * q[row][h] . key), over the tokens up to the row's own (and, with
+ * window > 0, the last `window` of those alone); query head h goes with head h / (q_heads / heads). scale 0: 1 / sqrt(dim). A row without any token:
+ * zeros. Tokens that a row does not see may hold anything. The same bits for the same inputs, whatever ran before. ws: qw_attn_ws_bytes of device memory, 16-byte aligned, which
+ * need not be cleared; one call at a time has it (calls one after another on one stream may share it, calls on two streams, or graphs that may run side by side, may not). */
+size_t qw_attn_ws_bytes(const qw_gpu *g, int dim);
+bool qw_attn(qw_batch *b, const qw_kv *c, const qw_kv_step *s, int q_heads, const qw_kv_rows *q, const qw_kv_rows *out, float scale, int window, const qw_at *ws);
+
+/* A recorder for callers with streams and memory of their own (a framework's tensors, a stream under graph capture): begin, any of the
+ * functions above, end. The launches go to `stream` (a hipStream_t of this device; NULL: the default stream), in order, and end returns without
+ * waiting; nothing is allocated, copied or synchronised. Buffers have to be device-only: qw_hip_buf_new_device, or views. One
+ * recorder at a time per device (NULL + qw_hip_last_error otherwise); qw_hip_stream_end gives it back and launches nothing where a function failed.
+ * qw_path_gg_moe_noalloc uses the same one. */
+qw_batch *qw_hip_stream_begin(qw_gpu *g, void *stream);
+bool qw_hip_stream_end(qw_batch *b);
+/* A buffer over [devptr, devptr + size) of device memory that somebody else owns and keeps: for the functions of this header alone (others refuse it).
+ * qw_buf_free frees the handle, not the memory. False + qw_hip_last_error: not memory of this device. */
+bool qw_hip_buf_view(qw_gpu *g, void *devptr, size_t size, qw_buf *out);
+
+#ifdef __cplusplus
+}
+#endif

@@ -6,8 +6,9 @@ Three steps, all cross-compile without a GPU:
   1. hipcc --genco: csrc/kernels/qw_kernels.hip -> csrc/qw_kernels_gfx950.hsaco (one code object: the same kernels spread over
      several measured 3 % slower on the 48-layer step), and a look at the waits in it that count loads (check_counted_waits);
      beside it the kernels for several launches in one -> csrc/qw_joined_gfx950.hsaco (kernels/qw_joined.hip.h says why they lie apart)
+     and those of the attention half of a step (kernels/qw_attn.hip) -> csrc/qw_attn_gfx950.hsaco
   2. hipcc -c: csrc/qw_noalloc.hip (host + device: the per-device scratch array of the entry point that allocates nothing) -> csrc/qw_noalloc.o
-  3. clang -std=c23: csrc/gpu_hip.c and csrc/qw_joined.c (embed the code objects) + csrc/qw_path.c + csrc/qw_gguf.c + csrc/qw_par.c + qw_noalloc.o -> qwental_amd/libqwgpu_hip.so
+  3. clang -std=c23: csrc/gpu_hip.c, csrc/qw_joined.c and csrc/qw_attn.c (embed the code objects) + csrc/qw_path.c + csrc/qw_gguf.c + csrc/qw_par.c + qw_noalloc.o -> qwental_amd/libqwgpu_hip.so
 """
 import concurrent.futures
 import heapq
@@ -33,6 +34,7 @@ if TAG:
     LIB = os.path.join(HERE, "libqwgpu_hip_%s.so" % TAG)
 HSACO = os.path.join(OBJDIR, "qw_kernels_gfx950.hsaco")
 JOINED = os.path.join(OBJDIR, "qw_joined_gfx950.hsaco")
+ATTN = os.path.join(OBJDIR, "qw_attn_gfx950.hsaco")
 PARTS, JOINED_PARTS = 0x3f, 0x40  # of qw_kernels.hip, groups of kernels in either code object
 # -packed-fp32-ops: packed FP32 instructions are kept out of every kernel of this library
 HIPFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("QW_BUILD_DEFS", "").split()
@@ -113,13 +115,16 @@ def check_counted_waits(text):
 
 def build(verbose=False, kernels=True):
     """kernels=False keeps the code object of the last build (host-side iterations: `python -m qwental_amd.build --host-only`)."""
-    if kernels or not (os.path.exists(HSACO) and os.path.exists(JOINED)):
+    attn = lambda: _run([HIPCC] + HIPFLAGS + ["--genco", "-I", os.path.join(CSRC, "kernels"), "-o", ATTN, os.path.join(CSRC, "kernels", "qw_attn.hip")])
+    if kernels or not (os.path.exists(HSACO) and os.path.exists(JOINED) and os.path.exists(ATTN)):
         genco = lambda out, parts: _run([HIPCC] + HIPFLAGS + parts + ["--genco", "-I", os.path.join(CSRC, "kernels"), "-o", out, os.path.join(CSRC, "kernels", "qw_kernels.hip")])
         some = any(f.startswith("-DQW_PARTS=") for f in HIPFLAGS)
-        with concurrent.futures.ThreadPoolExecutor(2) as two:
+        with concurrent.futures.ThreadPoolExecutor(3) as two:
+            third = two.submit(attn)
             for out in two.map(genco, (HSACO, JOINED), ([] if some else ["-DQW_PARTS=%d" % PARTS], ["-UQW_PARTS", "-DQW_PARTS=%d" % JOINED_PARTS])):
                 if verbose and out.strip():
                     print(out)
+            third.result()
         for k in COUNTING:
             text = listing(k)
             if text.strip() or not TAG:  # (a working build may hold some groups of kernels only)
@@ -127,8 +132,8 @@ def build(verbose=False, kernels=True):
     noalloc_o = os.path.join(OBJDIR, "qw_noalloc.o")
     _run([HIPCC] + HIPFLAGS + ["-fPIC", "-I", CSRC, "-I", os.path.join(ROOT, "include"), "-c", os.path.join(CSRC, "qw_noalloc.hip"), "-o", noalloc_o])
     out = _run([CLANG, "-std=c23", "-O2", "-Wall", "-Wextra", "-fPIC", "-shared", "--embed-dir=" + OBJDIR] + [f for f in os.environ.get("QW_BUILD_DEFS", "").split() if f.startswith("-D")] + ["-I", os.path.join(ROOT, "include"), "-I", CSRC,
-                "-I", os.path.join(ROCM, "include"), os.path.join(CSRC, "gpu_hip.c"), os.path.join(CSRC, "qw_joined.c"), os.path.join(CSRC, "qw_path.c"), os.path.join(CSRC, "qw_gguf.c"), os.path.join(CSRC, "qw_par.c"), noalloc_o, "-pthread", "-o", LIB,
-                "-L", os.path.join(ROCM, "lib"), "-lamdhip64", "-Wl,-rpath," + os.path.join(ROCM, "lib")])
+                "-I", os.path.join(ROCM, "include"), os.path.join(CSRC, "gpu_hip.c"), os.path.join(CSRC, "qw_joined.c"), os.path.join(CSRC, "qw_attn.c"), os.path.join(CSRC, "qw_path.c"), os.path.join(CSRC, "qw_gguf.c"), os.path.join(CSRC, "qw_par.c"), noalloc_o, "-pthread", "-o", LIB,
+                "-L", os.path.join(ROCM, "lib"), "-lamdhip64", "-lm", "-Wl,-rpath," + os.path.join(ROCM, "lib")])
     if verbose and out.strip():
         print(out)
     if TAG:

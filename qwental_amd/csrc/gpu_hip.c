@@ -11,9 +11,12 @@
 #define __HIP_PLATFORM_AMD__ 1
 #include "gpu.h"
 #include "qw_hip_ext.h"
+#include "qw_attn.h"
 #include "qw_internal.h"
+#include "kernels/qw_attn_kargs.h"
 #include "kernels/qw_kargs.h"
 #include <hip/hip_runtime_api.h>
+#include <math.h>
 #include <pthread.h>
 #include <stdarg.h>
 #include <stddef.h>
@@ -27,6 +30,7 @@ static const unsigned char qw_code_object[] = {
 #embed <qw_kernels_gfx950.hsaco>
 };
 extern const unsigned char qw_joined_object[]; // (qw_joined.c)
+extern const unsigned char qw_attn_object[];   // (qw_attn.c)
 
 #define QW_DNQ_MIN_DEFAULT 2u // token count from which down + combine run as one launch of token quarters (qwk_dnq_*)
 enum { QW_MAX_ARGS = 448, QW_MAX_KERNELS = 4096, QW_MAX_BIND = 32, QW_MAX_BYTES = 256, QW_PROF_MAX = 8192, QW_MAX_FUNCS = 256 };
@@ -38,6 +42,7 @@ typedef enum {
     FAM_BW_CHUNKS, FAM_BW_ROWS, // read pattern of a decode layer (bench/moe_bw.c)
     FAM_HC_DOWN, FAM_HC_MID, FAM_HC_UP, FAM_HC_UPV, // hyper-connection of the GGUF profile (kernels/hyper_gg.metal)
     FAM_PK_COUNT, FAM_PK_PLAN, FAM_PK_PLAN_T, FAM_PK_SCATTER, FAM_PK_ACT, FAM_PK_ACT2, FAM_PK_COMBINE, FAM_PK_ZERO, FAM_PF, // ragged packing and the grouped product
+    FAM_KV_WRITE, FAM_KV_READ, FAM_ATTN, // the attention half of a decode step (qw_attn.h)
 } qw_family;
 
 typedef struct { // parameters taken from the define block
@@ -76,6 +81,7 @@ typedef struct qw_hbuf {
     bool written;    // some dispatch has bound it in an output role
     unsigned nwriters, nslots; // dispatches of the batch being submitted that write it, and launches that can write the shadow for them (count_writers)
     bool apart;      // those several dispatches may all write the shadow themselves
+    bool view;       // somebody else's memory (qw_hip_buf_view)
     bool released;   // the device bytes were freed (qw_hip_buf_release_source): dptr is only the key of its tile-major copies
 } qw_hbuf;
 
@@ -153,6 +159,8 @@ struct qw_batch {
     bool noalloc;      // the device's static recorder (qw_hip_batch_begin_static): fixed storage, no tile-major copies made
     bool allow_released; // set by a translator while it binds weights that a tile-major copy may stand in for
     hipStream_t xstream; // noalloc: the caller's stream (NULL: the device's)
+    bool own_stream;   // xstream as it is, NULL being HIP's default stream (qw_hip_stream_begin)
+    int restore_dev;   // the caller's current device, where it is another one
     uint64_t seq;      // this batch's number (qw_hbuf.out_seq)
     qw_hbuf **outs;    // buffers whose pending_out this batch raised
     int nouts, capouts;
@@ -220,6 +228,9 @@ static const qw_wg_rule wg_rules[] = {
     {"qwk_moe_prep_slices", QW_WG_PREP_SLICES, 0, 0},
     {"qwk_moe_prep", QW_WG_PREP, 0, 0},
     {"qwk_hc_up", QW_WG_HC_UP, 0, 0},
+    {"qwk_attn_join", QW_WG_JOIN, 0, 0},
+    {"qwk_attn_", QW_WG_ATTN, 0, 0},
+    {"qwk_kv_", QW_WG_KV, 0, 0},
 };
 static const qw_wg_rule *wg_rule(const char *fname) {
     static const qw_wg_rule any = {"", 0, 0, 0};
@@ -235,7 +246,8 @@ struct qw_gpu {
     char name[256];
     size_t total_mem;
     int ncu;
-    hipModule_t mod, joined; // the kernels, and the forms of some of them for several launches in one
+    hipModule_t mod, joined, attn; // the kernels, the forms of some of them for several launches in one, and those of qw_attn.h
+    struct qw_kernel *attn_k[QW_ATTN_CALLS];
     void *tabs;   // this backend's own lookup tables in HBM (QW_TAB_BYTES); the pre-signed IQ3_S table sits at QW_TAB_IQ3SS
     hipStream_t stream[2];
     int cur_stream;
@@ -357,7 +369,8 @@ static hipFunction_t find_func_in(hipModule_t mod, const char *fname) {
     (void)hipGetLastError();
     return NULL;
 }
-static hipFunction_t find_func(qw_gpu *g, const char *fname) { return find_func_in(g->mod, fname); }
+static bool of_attn(const char *fname) { return !strncmp(fname, "qwk_attn_", 9) || !strncmp(fname, "qwk_kv_", 7); }
+static hipFunction_t find_func(qw_gpu *g, const char *fname) { return find_func_in(of_attn(fname) ? g->attn : g->mod, fname); }
 
 // ---------------------------------------------------------------- device
 // n bytes into HBM by stores of the host; returns a word whose reading back says that they have arrived.
@@ -402,7 +415,8 @@ qw_gpu *qw_gpu_open(void) {
         free(g);
         return NULL;
     }
-    if (hipModuleLoadData(&g->mod, qw_code_object) != hipSuccess || hipModuleLoadData(&g->joined, qw_joined_object) != hipSuccess) {
+    if (hipModuleLoadData(&g->mod, qw_code_object) != hipSuccess || hipModuleLoadData(&g->joined, qw_joined_object) != hipSuccess ||
+        hipModuleLoadData(&g->attn, qw_attn_object) != hipSuccess) {
         fprintf(stderr, "qw_gpu_open: the embedded gfx950 code objects do not load\n");
         free(g);
         return NULL;
@@ -503,6 +517,7 @@ void qw_gpu_close(qw_gpu *g) {
     if (g->na_batch) { free(g->na_batch->l); free(g->na_batch->use); free(g->na_batch); }
     (void)hipModuleUnload(g->mod);
     (void)hipModuleUnload(g->joined);
+    (void)hipModuleUnload(g->attn);
     free(g->kernels);
     free(g);
 }
@@ -761,6 +776,11 @@ bool qw_gpu_compile(qw_gpu *g, const char *src, size_t len, char *err, size_t er
         // checked when it is dispatched (the other one's are placeholders).
         if (!reg_kernel(g, d, n, "bw_chunks", FAM_BW_CHUNKS, &p, err, errlen) || !reg_kernel(g, d, n, "bw_rows", FAM_BW_ROWS, &p, err, errlen)) { ok = false; goto out; }
     }
+    if (def_get(d, n, "QW_ATTN")) { // include/qw_attn.h: sizes come with the dispatch
+        p = (qw_kparams){0};
+        if (!reg_kernel(g, d, n, "kv_write", FAM_KV_WRITE, &p, err, errlen) || !reg_kernel(g, d, n, "kv_read", FAM_KV_READ, &p, err, errlen) ||
+            !reg_kernel(g, d, n, "attn_paged", FAM_ATTN, &p, err, errlen)) { ok = false; goto out; }
+    }
     if (def_get(d, n, "QW_HIP_MEM")) { // this backend's own measurement helpers
         p = (qw_kparams){0};
         if (!reg_kernel(g, d, n, "qw_bw_read", FAM_BW_READ, &p, err, errlen) || !reg_kernel(g, d, n, "qw_copy", FAM_COPY, &p, err, errlen) ||
@@ -884,7 +904,7 @@ void qw_buf_free(qw_buf *b) {
     if (!b || !b->handle) return;
     qw_hbuf *h = b->handle;
     packs_drop(h);
-    if (!h->released) (void)hipFree(h->dptr);
+    if (!h->released && !h->view) (void)hipFree(h->dptr);
     if (h->own_host) {
         if (h->pinned) (void)hipHostFree(h->host);
         else free(h->host);
@@ -1143,12 +1163,15 @@ static bool fail(qw_batch *b, const char *fmt, ...) {
     return false;
 }
 
+static bool of_attn_family(qw_family f) { return f == FAM_KV_WRITE || f == FAM_KV_READ || f == FAM_ATTN; }
 // Binding `index` as a device pointer with at least `need` bytes after its offset; records the use.
 static bool bind_ptr(qw_batch *b, unsigned index, size_t need, bool out, const char *what, void **p) {
     qw_hbuf *h = b->buf[index].h;
     if (!h) return fail(b, "%s: nothing bound at index %u (%s)", b->k->name, index, what);
     const size_t off = b->buf[index].off;
     if (off > h->size || need > h->size - off) return fail(b, "%s: %s at index %u needs %zu bytes after offset %zu, buffer has %zu", b->k->name, what, index, need, off, h->size);
+    if (h->view && !of_attn_family(b->k->fam)) return fail(b, "%s: %s at index %u is a view of foreign memory (qw_hip_buf_view): for the functions of qw_attn.h", b->k->name, what, index);
+    if (b->own_stream && !h->device_only) return fail(b, "%s: %s at index %u has a host side: a recorder on a stream takes device-only buffers and views", b->k->name, what, index);
     if (out && h->wrapped) return fail(b, "%s: %s at index %u is a wrapped (read-only) buffer", b->k->name, what, index);
     if (h->released && (out || !b->allow_released))
         return fail(b, "%s: %s at index %u: the buffer's GGUF-order bytes were released (qw_hip_buf_release_source); only dispatches that a tile-major copy serves may bind it", b->k->name, what, index);
@@ -2429,6 +2452,120 @@ static bool tr_fill_blocks(qw_batch *b) {
     return add_launch(b, "qwk_fill_blocks", (unsigned)(wg < 65536 ? wg : 65536), 256, &a, sizeof a);
 }
 
+// ---------------------------------------------------------------- the attention half of a decode step (include/qw_attn.h)
+// Bindings: 0 cache, 1 first, 2 len, 3 table, 4 q, 5 q_out or out, 6 k or ws, 7 v, 8 freq, 9 pos, 10 qw_attn_geo.
+typedef struct { const char *p; size_t stride, width, rows; } qw_span; // rows of width bytes
+static size_t span_bytes(const qw_span *s) { return (s->rows - 1) * s->stride + s->width; }
+// Whether two spans share a byte, as far as it can be told: with one stride by the rows' places in it, with two by their whole ranges.
+static bool meet(const qw_span *x, const qw_span *y) {
+    if (!x->p || !y->p || x->p + span_bytes(x) <= y->p || y->p + span_bytes(y) <= x->p) return false;
+    if (x->stride != y->stride) return true;
+    const size_t d = x->p < y->p ? (size_t)(y->p - x->p) % x->stride : (x->stride - (size_t)(x->p - y->p) % x->stride) % x->stride;
+    return d < x->width || d + y->width > x->stride;
+}
+static bool apart(qw_batch *b, const qw_span *x, const char *xs, const qw_span *y, const char *ys) { return !meet(x, y) || fail(b, "%s: %s and %s overlap", b->k->name, xs, ys); }
+// The binary16 rows at `index`: heads of dim values, checked and bound.
+static bool kv_rows(qw_batch *b, unsigned index, bool out, const qw_attn_geo *x, int heads, int32_t stride, const char *what, uint16_t **p, uint32_t *str, qw_span *s) {
+    const int64_t width = (int64_t)heads * x->dim;
+    if (stride == 0) stride = (int32_t)width;
+    if (stride < width || stride % 8) return fail(b, "%s: %s: %d values from row to row (a multiple of 8, at least %lld)", b->k->name, what, stride, (long long)width);
+    *s = (qw_span){.stride = (size_t)stride * 2, .width = (size_t)width * 2, .rows = (size_t)x->rows};
+    if (!bind_ptr(b, index, span_bytes(s), out, what, (void **)p)) return false;
+    if ((uintptr_t)*p % 16) return fail(b, "%s: %s must be 16-byte aligned", b->k->name, what);
+    s->p = (const char *)*p;
+    *str = (uint32_t)stride;
+    return true;
+}
+static bool kv_bind(qw_batch *b, qw_attn_geo *x, qwk_kv *c, bool write, qw_span *cache) {
+    if (!bind_bytes(b, QW_ATTN_GEO, x, sizeof *x, "sizes")) return false;
+    const size_t bytes = qw_kv_bytes(x->type, x->heads, x->dim, x->page, x->pages);
+    if (!bytes) return fail(b, "%s: a cache of type %d, %d heads of %d values, %d pages of %d tokens (types 1 and 8, 1 to %d heads of 64, 128, 192 or 256 values, pages of a power of two from 16 to %d)", b->k->name, x->type,
+                            x->heads, x->dim, x->pages, x->page, QW_ATTN_MAX_HEADS, QW_ATTN_MAX_PAGE);
+    if (x->slots < 1 || x->slots > QW_KV_MAX_SLOTS || x->rows < 1 || x->rows > QW_KV_MAX_ROWS) return fail(b, "%s: %d slots, %d rows (1 to %d, 1 to %d)", b->k->name, x->slots, x->rows, QW_KV_MAX_SLOTS, QW_KV_MAX_ROWS);
+    if (x->max_pages < 1 || (int64_t)x->max_pages * x->page > INT32_MAX / 2) return fail(b, "%s: %d pages a slot of %d tokens (up to 2^30 tokens)", b->k->name, x->max_pages, x->page);
+    *c = (qwk_kv){.slots = (uint32_t)x->slots, .rows = (uint32_t)x->rows, .max_pages = (uint32_t)x->max_pages, .pages = (uint32_t)x->pages, .page_log2 = (uint32_t)__builtin_ctz((unsigned)x->page), .heads = (uint32_t)x->heads,
+                  .dim = (uint32_t)x->dim, .unit = (uint32_t)(x->dim * (x->type == 1 ? 64 : 34)), .page_bytes = bytes / (size_t)x->pages};
+    if (!bind_ptr(b, 0, bytes, write, "cache", (void **)&c->cache) || !bind_ptr(b, 1, ((size_t)x->slots + 1) * 4, false, "first", (void **)&c->first) || !bind_ptr(b, 2, (size_t)x->slots * 4, false, "len", (void **)&c->len) ||
+        !bind_ptr(b, 3, (size_t)x->slots * (size_t)x->max_pages * 4, false, "table", (void **)&c->table)) return false;
+    if ((uintptr_t)c->cache % 16 || (uintptr_t)c->first % 4 || (uintptr_t)c->len % 4 || (uintptr_t)c->table % 4) return fail(b, "%s: cache, first, len and table must be 16- and 4-byte aligned", b->k->name);
+    *cache = (qw_span){(const char *)c->cache, bytes, bytes, 1};
+    return true;
+}
+static bool tr_kv_write(qw_batch *b) {
+    qw_attn_geo x;
+    qwk_kv_write_args a = {0};
+    qw_span cache, q = {0}, qo = {0}, k, v;
+    if (!kv_bind(b, &x, &a.c, true, &cache)) return false;
+    if (x.q_heads < 0 || x.q_heads > QW_ATTN_MAX_Q_HEADS) return fail(b, "kv_write: %d query heads (0 to %d)", x.q_heads, QW_ATTN_MAX_Q_HEADS);
+    if (x.q_heads && (!kv_rows(b, 4, false, &x, x.q_heads, x.stride[0], "q", (uint16_t **)&a.q, &a.q_stride, &q) || !kv_rows(b, 5, true, &x, x.q_heads, x.stride[1], "q_out", &a.q_out, &a.qo_stride, &qo))) return false;
+    if (!kv_rows(b, 6, false, &x, x.heads, x.stride[2], "k", (uint16_t **)&a.k, &a.k_stride, &k) || !kv_rows(b, 7, false, &x, x.heads, x.stride[3], "v", (uint16_t **)&a.v, &a.v_stride, &v)) return false;
+    if (x.rot < 0 || x.rot > x.dim || x.rot % 2) return fail(b, "kv_write: %d values of %d turn (an even number)", x.rot, x.dim);
+    if (x.rot) {
+        if (x.axes != 1 && x.axes != 3) return fail(b, "kv_write: positions in %d axes (1 or 3)", x.axes);
+        if (x.axes == 3 && (x.pairs[0] < 0 || x.pairs[1] < 0 || x.pairs[2] < 0 || (int64_t)x.pairs[0] + x.pairs[1] + x.pairs[2] != x.rot / 2))
+            return fail(b, "kv_write: %d + %d + %d pairs of values for %d", x.pairs[0], x.pairs[1], x.pairs[2], x.rot);
+        if (!bind_ptr(b, 8, (size_t)x.rot / 2 * 8, false, "freq", (void **)&a.freq) || !bind_ptr(b, 9, (size_t)x.rows * (size_t)x.axes * 4, false, "pos", (void **)&a.pos)) return false;
+        if ((uintptr_t)a.freq % 8 || (uintptr_t)a.pos % 4) return fail(b, "kv_write: freq and pos must be 8- and 4-byte aligned");
+    }
+    // q_out may be q: a wave has read a head before it writes it
+    if (qo.p && !(qo.p == q.p && qo.stride == q.stride) && !apart(b, &qo, "q_out", &q, "q")) return false;
+    if (!apart(b, &qo, "q_out", &k, "k") || !apart(b, &qo, "q_out", &v, "v") || !apart(b, &qo, "q_out", &cache, "the cache") || !apart(b, &q, "q", &cache, "the cache") || !apart(b, &k, "k", &cache, "the cache") ||
+        !apart(b, &v, "v", &cache, "the cache")) return false;
+    a.q_heads = (uint32_t)x.q_heads, a.rot = (uint32_t)x.rot, a.axes = (uint32_t)x.axes, a.pairs0 = (uint32_t)x.pairs[0], a.pairs1 = (uint32_t)x.pairs[1], a.adjacent = x.adjacent != 0;
+    if (!add_launch(b, x.type == 1 ? "qwk_kv_write_f1" : "qwk_kv_write_f8", (unsigned)x.rows, QW_WG_KV, &a, sizeof a)) return false;
+    b->l[b->nl - 1].gy = cdiv((unsigned)(x.q_heads + 2 * x.heads), QW_WG_KV / 64);
+    return true;
+}
+static bool tr_kv_read(qw_batch *b) {
+    qw_attn_geo x;
+    qwk_kv_read_args a = {0};
+    qw_span cache, k, v;
+    if (!kv_bind(b, &x, &a.c, false, &cache)) return false;
+    if (!kv_rows(b, 6, true, &x, x.heads, x.stride[2], "k", &a.k, &a.k_stride, &k) || !kv_rows(b, 7, true, &x, x.heads, x.stride[3], "v", &a.v, &a.v_stride, &v)) return false;
+    if (!apart(b, &k, "k", &v, "v") || !apart(b, &k, "k", &cache, "the cache") || !apart(b, &v, "v", &cache, "the cache")) return false;
+    if (!add_launch(b, x.type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", (unsigned)x.rows, QW_WG_KV, &a, sizeof a)) return false;
+    b->l[b->nl - 1].gy = cdiv((unsigned)x.heads, QW_WG_KV / 64);
+    return true;
+}
+// Two workgroups a compute unit; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
+static unsigned attn_grid(const qw_gpu *g) { return 2 * (unsigned)g->ncu; }
+static size_t attn_part_bytes(const qw_gpu *g, int dim, unsigned qt) { return (size_t)attn_grid(g) * 2 * 16 * qt * (size_t)dim * 4; }
+size_t qw_attn_ws_bytes(const qw_gpu *g, int dim) { return !g || dim < 64 || dim > 256 || dim % 64 ? 0 : attn_part_bytes(g, dim, 2) + attn_part_bytes(g, 2, 2); }
+static bool tr_attn(qw_batch *b) {
+    static const char *const names[2][4][2] = {{{"qwk_attn_f1_d64_q1", "qwk_attn_f1_d64_q2"}, {"qwk_attn_f1_d128_q1", "qwk_attn_f1_d128_q2"}, {"qwk_attn_f1_d192_q1", "qwk_attn_f1_d192_q2"}, {"qwk_attn_f1_d256_q1", "qwk_attn_f1_d256_q2"}},
+                                               {{"qwk_attn_f8_d64_q1", "qwk_attn_f8_d64_q2"}, {"qwk_attn_f8_d128_q1", "qwk_attn_f8_d128_q2"}, {"qwk_attn_f8_d192_q1", "qwk_attn_f8_d192_q2"}, {"qwk_attn_f8_d256_q1", "qwk_attn_f8_d256_q2"}}};
+    qw_attn_geo x;
+    qwk_attn_args a = {0};
+    qw_span cache, q, out, ws;
+    if (!kv_bind(b, &x, &a.c, false, &cache)) return false;
+    if (x.q_heads < 1 || x.q_heads > QW_ATTN_MAX_Q_HEADS || x.q_heads % x.heads) return fail(b, "attn_paged: %d query heads for %d of keys (a multiple, up to %d)", x.q_heads, x.heads, QW_ATTN_MAX_Q_HEADS);
+    if (x.window < 0 || !(x.scale >= 0) || x.scale > 1e30f) return fail(b, "attn_paged: window %d, scale %g", x.window, (double)x.scale);
+    if (!kv_rows(b, 4, false, &x, x.q_heads, x.stride[0], "q", (uint16_t **)&a.q, &a.q_stride, &q) || !kv_rows(b, 5, true, &x, x.q_heads, x.stride[1], "out", &a.out, &a.out_stride, &out)) return false;
+    const size_t need = qw_attn_ws_bytes(b->g, x.dim);
+    if (!bind_ptr(b, 6, need, true, "workspace", (void **)&a.part)) return false;
+    if ((uintptr_t)a.part % 16) return fail(b, "attn_paged: the workspace must be 16-byte aligned");
+    ws = (qw_span){(const char *)a.part, need, need, 1};
+    if (!apart(b, &out, "out", &q, "q") || !apart(b, &out, "out", &cache, "the cache") || !apart(b, &ws, "the workspace", &q, "q") || !apart(b, &ws, "the workspace", &out, "out") || !apart(b, &ws, "the workspace", &cache, "the cache"))
+        return false;
+    a.group = (uint32_t)(x.q_heads / x.heads), a.window = (uint32_t)x.window, a.grid = attn_grid(b->g);
+    a.scale = (x.scale > 0 ? x.scale : 1 / sqrtf((float)x.dim)) * 1.44269504f;
+    // rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode
+    const unsigned qt = cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
+    a.ml = a.part + attn_part_bytes(b->g, x.dim, 2) / 4;
+    if (!add_launch(b, names[x.type == 8][x.dim / 64 - 1][qt - 1], a.grid, QW_WG_ATTN, &a, sizeof a)) return false;
+    if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", (unsigned)x.rows, QW_WG_JOIN, &a, sizeof a)) return false;
+    b->l[b->nl - 1].gy = (unsigned)x.dim / 64, b->l[b->nl - 1].gz = (unsigned)x.q_heads;
+    return true;
+}
+qw_kernel *qw_hip_attn_kernel(qw_batch *b, int which) {
+    static const char *const names[QW_ATTN_CALLS] = {"kv_write", "kv_read", "attn_paged"}, def[] = "#define QW_ATTN 1\n";
+    qw_gpu *g = b->g;
+    if (!g->attn_k[which] && qw_gpu_compile(g, def, sizeof def - 1, NULL, 0))
+        for (int i = 0; i < QW_ATTN_CALLS; i++) g->attn_k[i] = qw_kernel_get(g, names[i]);
+    return g->attn_k[which];
+}
+bool qw_hip_batch_failed(const qw_batch *b) { return b->failed; }
+
 void qw_batch_dispatch(qw_batch *b, unsigned gx, unsigned gy, unsigned gz, unsigned tx, unsigned ty, unsigned tz) {
     (void)gz; (void)tx; (void)ty; (void)tz;
     if (b->failed) return;
@@ -2465,6 +2602,9 @@ void qw_batch_dispatch(qw_batch *b, unsigned gx, unsigned gy, unsigned gz, unsig
     case FAM_PK_ACT2: ok = tr_pk_act2(b); break;
     case FAM_PK_COMBINE: ok = tr_pk_combine(b, gy); break;
     case FAM_PF: ok = tr_pf(b, gy); break;
+    case FAM_KV_WRITE: ok = tr_kv_write(b); break;
+    case FAM_KV_READ: ok = tr_kv_read(b); break;
+    case FAM_ATTN: ok = tr_attn(b); break;
     default: ok = tr_mem(b, gx);
     }
     if (ok && b->nl > first) b->l[b->nl - 1].last_of_dispatch = true;
@@ -3138,7 +3278,7 @@ qw_batch *qw_hip_batch_begin_static(qw_gpu *g, void *stream) {
 }
 bool qw_hip_batch_launch_static(qw_batch *b, bool recorded) {
     qw_gpu *g = b->g;
-    hipStream_t st = b->xstream ? b->xstream : g->stream[b->stream];
+    hipStream_t st = b->xstream || b->own_stream ? b->xstream : g->stream[b->stream];
     bool ok = recorded && !b->failed && flush_select(b) && flush_tw(b, NULL, NULL) && flush_pf(b) && flush_gu(b) && flush_dn(b) && flush_pk(b) && !b->failed;
     for (int i = 0; ok && i < b->nl; i++) {
         qw_launch *l = &b->l[i];
@@ -3147,6 +3287,57 @@ bool qw_hip_batch_launch_static(qw_batch *b, bool recorded) {
     }
     g->na_busy = false;
     return ok;
+}
+
+// The same for callers from outside, whose device may not be the current one.
+qw_batch *qw_hip_stream_begin(qw_gpu *g, void *stream) {
+    if (!g) return NULL;
+    int cur = g->dev;
+    hipDevice_t of = g->dev;
+    if (stream && (hipStreamGetDevice((hipStream_t)stream, &of) != hipSuccess || of != g->dev)) {
+        (void)hipGetLastError();
+        set_err(g, "qw_hip_stream_begin: not a stream of device %d", g->dev);
+        return NULL;
+    }
+    if (!HIPOK(g, hipGetDevice(&cur)) || (cur != g->dev && !HIPOK(g, hipSetDevice(g->dev)))) return NULL;
+    qw_batch *b = qw_hip_batch_begin_static(g, stream);
+    if (!b) {
+        if (cur != g->dev) (void)hipSetDevice(cur);
+        set_err(g, "qw_hip_stream_begin: the device's fixed recorder is missing or in use");
+        return NULL;
+    }
+    b->own_stream = true, b->restore_dev = cur;
+    return b;
+}
+bool qw_hip_stream_end(qw_batch *b) {
+    if (!b) return false;
+    qw_gpu *g = b->g;
+    const int cur = b->restore_dev;
+    const bool ok = qw_hip_batch_launch_static(b, true);
+    if (cur != g->dev) (void)hipSetDevice(cur);
+    return ok;
+}
+bool qw_hip_buf_view(qw_gpu *g, void *devptr, size_t size, qw_buf *out) {
+    if (!g || !out) return false;
+    *out = (qw_buf){0};
+    hipPointerAttribute_t at;
+    if (!devptr || hipPointerGetAttributes(&at, devptr) != hipSuccess || at.type != hipMemoryTypeDevice || at.device != g->dev) {
+        (void)hipGetLastError();
+        set_err(g, "qw_hip_buf_view: %p is not memory of device %d", devptr, g->dev);
+        return false;
+    }
+    hipDeviceptr_t base = NULL;
+    size_t bytes = 0;
+    if (hipMemGetAddressRange(&base, &bytes, devptr) != hipSuccess || size > bytes - (size_t)((char *)devptr - (char *)base)) {
+        (void)hipGetLastError();
+        set_err(g, "qw_hip_buf_view: %zu bytes from %p on end beyond their allocation", size, devptr);
+        return false;
+    }
+    qw_hip_view *v = calloc(1, sizeof *v);
+    if (!v) return false;
+    qw_hip_view_init(g, v, devptr, size, out);
+    ((qw_hbuf *)out->handle)->view = true;
+    return true;
 }
 
 // ---------------------------------------------------------------- profiling and bench utilities

@@ -1,0 +1,51 @@
+/* Argument records of the kernels of a decode step's attention and sampling (qw_attn.hip), shared with the host. Plain C. */
+#pragma once
+#include <stdint.h>
+
+#define QW_UNIT 16u           /* tokens of a unit: what the cache's layout is made of */
+#define QW_ATTN_TILE 32u      /* tokens by which the work is shared out */
+#define QW_WG_ATTN 256u       /* four waves, each with tiles of its own */
+#define QW_WG_JOIN 256u
+#define QW_WG_KV 256u
+#define QW_KV_SLOTS_MAX 256u  /* a thread of a workgroup for each */
+
+typedef struct { /* a layer's cache and a step's rows, as every kernel of them takes them */
+    uint8_t *cache;
+    const uint32_t *first, *len, *table;
+    uint64_t page_bytes;
+    uint32_t slots, rows, max_pages, pages, page_log2, heads, dim, unit; /* unit: bytes */
+} qwk_kv;
+
+typedef struct {
+    qwk_kv c;
+    const uint16_t *q;
+    uint16_t *out;
+    float *part, *ml; /* partial results: [2 grid][16 QT][dim], and of each row its maximum and its sum */
+    uint32_t q_stride, out_stride, group, window, grid;
+    float scale; /* of a score, log2(e) in it */
+} qwk_attn_args;
+
+typedef struct {
+    qwk_kv c;
+    const uint16_t *q, *k, *v;
+    uint16_t *q_out;
+    const double *freq;
+    const int32_t *pos;
+    uint32_t q_stride, qo_stride, k_stride, v_stride, q_heads, rot, axes, pairs0, pairs1, adjacent;
+} qwk_kv_write_args;
+
+typedef struct {
+    qwk_kv c;
+    uint16_t *k, *v;
+    uint32_t k_stride, v_stride;
+} qwk_kv_read_args;
+
+/* What the functions of include/qw_attn.h hand a dispatch beside its buffers, as inline bytes at index QW_ATTN_GEO. */
+#define QW_ATTN_GEO 10u
+typedef struct {
+    int32_t type, heads, dim, page, pages, slots, rows, max_pages, q_heads;
+    int32_t stride[4]; /* q, q_out or out, k, v */
+    int32_t window;
+    float scale;
+    int32_t rot, axes, pairs[3], adjacent;
+} qw_attn_geo;

@@ -1,0 +1,63 @@
+// Host side of the attention half of a decode step (include/qw_attn.h): bindings and sizes of each call. What they have to be is checked where the
+// dispatches are translated (gpu_hip.c). The kernels' code object is embedded here, beside the others.
+#include "qw_attn.h"
+#include "qw_hip_ext.h"
+#include "qw_internal.h"
+#include "kernels/qw_attn_kargs.h"
+
+QW_INTERNAL extern const unsigned char qw_attn_object[];
+const unsigned char qw_attn_object[] = {
+#embed <qw_attn_gfx950.hsaco>
+};
+
+static bool log2_of(int x, uint32_t *l) {
+    if (x < 1 || (x & (x - 1))) return false;
+    *l = (uint32_t)__builtin_ctz((unsigned)x);
+    return true;
+}
+size_t qw_kv_bytes(int type, int heads, int dim, int page, int pages) {
+    uint32_t l;
+    if ((type != 1 && type != 8) || heads < 1 || heads > QW_ATTN_MAX_HEADS || dim < 64 || dim > 256 || dim % 64 || page < (int)QW_UNIT || page > QW_ATTN_MAX_PAGE || !log2_of(page, &l) || pages < 1) return 0;
+    return (size_t)pages * (size_t)heads * (size_t)(page / (int)QW_UNIT) * (size_t)(dim * (type == 1 ? 64 : 34));
+}
+
+static void bind(qw_batch *b, unsigned index, const qw_at *at) { qw_batch_buf(b, index, at ? at->buf : NULL, at ? at->offset : 0); }
+static qw_attn_geo begin(qw_batch *b, int which, const qw_kv *c, const qw_kv_step *s) {
+    qw_batch_kernel(b, qw_hip_attn_kernel(b, which));
+    bind(b, 0, &c->at), bind(b, 1, &s->first), bind(b, 2, &s->len), bind(b, 3, &s->table);
+    return (qw_attn_geo){.type = c->type, .heads = c->heads, .dim = c->dim, .page = c->page, .pages = c->pages, .slots = s->slots, .rows = s->rows, .max_pages = s->max_pages};
+}
+static void rows_at(qw_batch *b, unsigned index, const qw_kv_rows *r, int32_t *stride) {
+    bind(b, index, r ? &r->at : NULL);
+    *stride = r ? r->stride : 0;
+}
+static bool end(qw_batch *b, const qw_attn_geo *geo) {
+    qw_batch_bytes(b, QW_ATTN_GEO, geo, sizeof *geo);
+    qw_batch_dispatch(b, 1, 1, 1, 1, 1, 1);
+    return !qw_hip_batch_failed(b);
+}
+
+bool qw_kv_write(qw_batch *b, const qw_kv *c, const qw_kv_step *s, const qw_rope *rope, int q_heads, const qw_kv_rows *q, const qw_kv_rows *q_out, const qw_kv_rows *k,
+                 const qw_kv_rows *v) {
+    if (!b || !c || !s) return false;
+    qw_attn_geo geo = begin(b, QW_ATTN_WRITE, c, s);
+    geo.q_heads = q_heads;
+    rows_at(b, 4, q, &geo.stride[0]), rows_at(b, 5, q_out, &geo.stride[1]), rows_at(b, 6, k, &geo.stride[2]), rows_at(b, 7, v, &geo.stride[3]);
+    bind(b, 8, rope ? &rope->freq : NULL), bind(b, 9, rope ? &rope->pos : NULL);
+    if (rope) geo.rot = rope->dims, geo.axes = rope->axes, geo.pairs[0] = rope->pairs[0], geo.pairs[1] = rope->pairs[1], geo.pairs[2] = rope->pairs[2], geo.adjacent = rope->adjacent;
+    return end(b, &geo);
+}
+bool qw_kv_read(qw_batch *b, const qw_kv *c, const qw_kv_step *s, const qw_kv_rows *k, const qw_kv_rows *v) {
+    if (!b || !c || !s) return false;
+    qw_attn_geo geo = begin(b, QW_ATTN_READ, c, s);
+    rows_at(b, 6, k, &geo.stride[2]), rows_at(b, 7, v, &geo.stride[3]);
+    return end(b, &geo);
+}
+bool qw_attn(qw_batch *b, const qw_kv *c, const qw_kv_step *s, int q_heads, const qw_kv_rows *q, const qw_kv_rows *out, float scale, int window, const qw_at *ws) {
+    if (!b || !c || !s) return false;
+    qw_attn_geo geo = begin(b, QW_ATTN_ATTN, c, s);
+    geo.q_heads = q_heads, geo.scale = scale, geo.window = window;
+    rows_at(b, 4, q, &geo.stride[0]), rows_at(b, 5, out, &geo.stride[1]);
+    bind(b, 6, ws);
+    return end(b, &geo);
+}

@@ -44,6 +44,15 @@ QW_INTERNAL bool qw_hip_batch_copies_to_come(const qw_batch *b);
 QW_INTERNAL bool qw_hip_batch_copies_made(const qw_batch *b);
 QW_INTERNAL double qw_hip_batch_end_parts(qw_batch *b, double *secs);
 
+/* The kernels of include/qw_attn.h: their code object (qw_attn.c), the kernel of a call (registered with the device at its first use), and whether a
+ * dispatch of the batch was refused. */
+enum { QW_ATTN_WRITE, QW_ATTN_READ, QW_ATTN_ATTN, QW_ATTN_CALLS };
+#define QW_ATTN_MAX_HEADS 256
+#define QW_ATTN_MAX_Q_HEADS 1024
+#define QW_ATTN_MAX_PAGE 65536
+QW_INTERNAL qw_kernel *qw_hip_attn_kernel(qw_batch *b, int which);
+QW_INTERNAL bool qw_hip_batch_failed(const qw_batch *b);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,6 @@
 """ctypes binding of libqwgpu_hip.so: the GPU interface (include/gpu.h), its HIP additions (include/qw_hip_ext.h),
-the host side of the path (include/qw_path.h), the GGUF reader (include/qw_gguf.h) and the step planner
-(include/qw_par.h). Thin by design: one Python
+the host side of the path (include/qw_path.h), the GGUF reader (include/qw_gguf.h), the step planner
+(include/qw_par.h) and, with attn.py, the attention half of a step (include/qw_attn.h). Thin by design: one Python
 method per C function."""
 import contextlib
 import ctypes as C
@@ -49,7 +49,7 @@ class QwGgufTensor(C.Structure):
                 ("offset", C.c_uint64), ("res_type", C.c_int)]
 
 
-# every symbol include/gpu.h, include/qw_hip_ext.h, include/qw_path.h and include/qw_gguf.h declare: (name, restype, argtypes)
+# every symbol include/gpu.h, include/qw_hip_ext.h, include/qw_path.h, include/qw_gguf.h and include/qw_par.h declare: (name, restype, argtypes)
 _vp, _sz, _u, _i, _b, _d = C.c_void_p, C.c_size_t, C.c_uint, C.c_int, C.c_bool, C.c_double
 _pb, _pt, _pm, _pg = C.POINTER(QwBuf), C.POINTER(QwTensor), C.POINTER(QwMoeLayer), C.POINTER(QwGgufTensor)
 _pi = C.POINTER(C.c_int)
@@ -115,6 +115,13 @@ SYMBOLS = [
     ("qw_par_want_slice", _b, [_vp, _i, _b, _d, C.POINTER(_d), _d, _d]),
 ]
 
+# include/qw_attn.h
+ATTN_SYMBOLS = [
+    ("qw_kv_bytes", _sz, [_i, _i, _i, _i, _i]), ("qw_kv_write", _b, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]), ("qw_kv_read", _b, [_vp, _vp, _vp, _vp, _vp]),
+    ("qw_attn_ws_bytes", _sz, [_vp, _i]), ("qw_attn", _b, [_vp, _vp, _vp, _i, _vp, _vp, C.c_float, _i, _vp]),
+    ("qw_hip_stream_begin", _vp, [_vp, _vp]), ("qw_hip_stream_end", _b, [_vp]), ("qw_hip_buf_view", _b, [_vp, _vp, _sz, _pb]),
+]
+
 
 def load_lib():
     """Load the built library; raises if it has not been built (python -m qwental_amd.build)."""
@@ -124,7 +131,7 @@ def load_lib():
     if not os.path.exists(lib_path()):
         raise RuntimeError("libqwgpu_hip.so is not built: run `python -m qwental_amd.build` (needs hipcc and clang from ROCm)")
     L = C.CDLL(lib_path())
-    for name, res, args in SYMBOLS:
+    for name, res, args in SYMBOLS + ATTN_SYMBOLS:
         if os.environ.get("QW_HIP_LIB") and not hasattr(L, name):
             continue  # another build of the library (experiments) may predate a symbol
         f = getattr(L, name)  # AttributeError if the library lacks a declared symbol
@@ -272,6 +279,35 @@ class Batch:
         return t
 
 
+class StreamBatch(Batch):
+    """A recorder on a stream of the caller's (include/qw_attn.h): end() launches and returns without waiting."""
+
+    def __init__(self, gpu, stream=None):
+        self.gpu, self.L = gpu, gpu.L
+        self.b = self.L.qw_hip_stream_begin(gpu.g, stream)
+        if not self.b:
+            raise RuntimeError(gpu.last_error())
+
+    def end(self):
+        b, self.b = self.b, None
+        if not self.L.qw_hip_stream_end(b):
+            raise RuntimeError("GPU launches failed: " + self.gpu.last_error())
+
+
+class View(Buf):
+    """A buffer over device memory that somebody else keeps (a tensor's, say)."""
+
+    def __init__(self, gpu, ptr, size):
+        self.gpu, self.L, self._keep = gpu, gpu.L, None
+        self.c = QwBuf()
+        if not self.L.qw_hip_buf_view(gpu.g, ptr, size, C.byref(self.c)):
+            raise RuntimeError(gpu.last_error())
+        self.size = self.c.size
+
+    def __del__(self):
+        self.free()
+
+
 class Gpu:
     def __init__(self):
         self.L = load_lib()
@@ -316,6 +352,13 @@ class Gpu:
 
     def batch(self, concurrent=False):
         return Batch(self, concurrent)
+
+    def stream(self, stream=None):
+        """A recorder on a hipStream_t (an integer; None or 0: the default stream)."""
+        return StreamBatch(self, stream)
+
+    def view(self, ptr, size):
+        return View(self, ptr, size)
 
     def profile(self, on):
         self.L.qw_profile_enable(self.g, on)
