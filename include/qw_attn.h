@@ -78,6 +78,17 @@ bool qw_kv_read(qw_batch *b, const qw_kv *c, const qw_kv_step *s, const qw_kv_ro
 size_t qw_attn_ws_bytes(const qw_gpu *g, int dim);
 bool qw_attn(qw_batch *b, const qw_kv *c, const qw_kv_step *s, int q_heads, const qw_kv_rows *q, const qw_kv_rows *out, float scale, int window, const qw_at *ws);
 
+/* One token a row of logits [rows][vocab] (float, `stride` values from row to row, 0: vocab; up to 2^20 of them). params: qw_sample_row [rows]; u: float [rows], random
+ * numbers in [0, 1) - the same ones give the same tokens. Of a row's tokens by falling logit (equal ones by their number), top_k (0: all) leaves the first
+ * top_k; top_p (1: all) as many of these as it takes to have top_p of their probability, at least one; min_p those of at least min_p times the largest probability. The token is the first one, by
+ * number, at which the sum of the probabilities of what is left exceeds u of its whole. Probabilities are softmax(logits / temperature); temperature 0: the first of the largest logits.
+ * NaN and minus infinity are never drawn; a row of nothing else gives 0xffffffff. ids: uint32 [rows]; probs (may be NULL): float [rows], the token's probability among
+ * those left. ws: qw_sample_ws_bytes of device memory, 16-byte aligned, as qw_attn's. */
+typedef struct { float temperature, top_p, min_p; uint32_t top_k; } qw_sample_row;
+#define QW_SAMPLE_MAX_VOCAB (1 << 20)
+size_t qw_sample_ws_bytes(const qw_gpu *g, int rows, int vocab);
+bool qw_sample(qw_batch *b, int rows, int vocab, int stride, const qw_at *logits, const qw_at *params, const qw_at *u, const qw_at *ids, const qw_at *probs, const qw_at *ws);
+
 /* A recorder for callers with streams and memory of their own (a framework's tensors, a stream under graph capture): begin, any of the
  * functions above, end. The launches go to `stream` (a hipStream_t of this device; NULL: the default stream), in order, and end returns without
  * waiting; nothing is allocated, copied or synchronised. Buffers have to be device-only: qw_hip_buf_new_device, or views. One

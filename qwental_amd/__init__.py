@@ -7,4 +7,4 @@ without a gfx950 device every entry point raises.
 """
 from . import synth  # noqa: F401
 from .gpu import Gpu, Buf, Path, Tensor, MoeLayer, Gguf, Par, lib_path, load_lib  # noqa: F401
-from .attn import Attn, KvCache, KvRead, KvStep, KvWrite, Rope, attn_ws_bytes, kv_bytes  # noqa: F401
+from .attn import Attn, KvCache, KvRead, KvStep, KvWrite, Rope, Sample, attn_ws_bytes, kv_bytes, sample_ws_bytes  # noqa: F401

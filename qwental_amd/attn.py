@@ -95,3 +95,14 @@ class KvRead(_Call):
 class Attn(_Call):
     def __init__(self, cache, step, q_heads, q, out, ws, scale=0.0, window=0, strides=(0, 0)):
         super().__init__("qw_attn", (cache, step, q, out, ws), cache.c, step.c, q_heads, _rows(q, strides[0]), _rows(out, strides[1]), scale, window, _at(ws))
+
+
+def sample_ws_bytes(gpu, rows, vocab):
+    return gpu.L.qw_sample_ws_bytes(gpu.g, rows, vocab)
+
+
+class Sample(_Call):
+    """One token a row. params: [rows] of (temperature, top-p, min-p: float32, top-k: uint32); u float32 [rows]; ids uint32 [rows]; probs float32 [rows] or None."""
+
+    def __init__(self, rows, vocab, logits, params, u, ids, probs, ws, stride=0):
+        super().__init__("qw_sample", (logits, params, u, ids, probs, ws), rows, vocab, stride, *(_at(x) if x is not None else None for x in (logits, params, u, ids, probs, ws)))

@@ -42,7 +42,7 @@ typedef enum {
     FAM_BW_CHUNKS, FAM_BW_ROWS, // read pattern of a decode layer (bench/moe_bw.c)
     FAM_HC_DOWN, FAM_HC_MID, FAM_HC_UP, FAM_HC_UPV, // hyper-connection of the GGUF profile (kernels/hyper_gg.metal)
     FAM_PK_COUNT, FAM_PK_PLAN, FAM_PK_PLAN_T, FAM_PK_SCATTER, FAM_PK_ACT, FAM_PK_ACT2, FAM_PK_COMBINE, FAM_PK_ZERO, FAM_PF, // ragged packing and the grouped product
-    FAM_KV_WRITE, FAM_KV_READ, FAM_ATTN, // the attention half of a decode step (qw_attn.h)
+    FAM_KV_WRITE, FAM_KV_READ, FAM_ATTN, FAM_SAMPLE, // the attention half of a decode step (qw_attn.h)
 } qw_family;
 
 typedef struct { // parameters taken from the define block
@@ -231,6 +231,7 @@ static const qw_wg_rule wg_rules[] = {
     {"qwk_attn_join", QW_WG_JOIN, 0, 0},
     {"qwk_attn_", QW_WG_ATTN, 0, 0},
     {"qwk_kv_", QW_WG_KV, 0, 0},
+    {"qwk_sample", QW_WG_SAMPLE, 0, 0},
 };
 static const qw_wg_rule *wg_rule(const char *fname) {
     static const qw_wg_rule any = {"", 0, 0, 0};
@@ -369,7 +370,7 @@ static hipFunction_t find_func_in(hipModule_t mod, const char *fname) {
     (void)hipGetLastError();
     return NULL;
 }
-static bool of_attn(const char *fname) { return !strncmp(fname, "qwk_attn_", 9) || !strncmp(fname, "qwk_kv_", 7); }
+static bool of_attn(const char *fname) { return !strncmp(fname, "qwk_attn_", 9) || !strncmp(fname, "qwk_kv_", 7) || !strncmp(fname, "qwk_sample", 10); }
 static hipFunction_t find_func(qw_gpu *g, const char *fname) { return find_func_in(of_attn(fname) ? g->attn : g->mod, fname); }
 
 // ---------------------------------------------------------------- device
@@ -779,7 +780,7 @@ bool qw_gpu_compile(qw_gpu *g, const char *src, size_t len, char *err, size_t er
     if (def_get(d, n, "QW_ATTN")) { // include/qw_attn.h: sizes come with the dispatch
         p = (qw_kparams){0};
         if (!reg_kernel(g, d, n, "kv_write", FAM_KV_WRITE, &p, err, errlen) || !reg_kernel(g, d, n, "kv_read", FAM_KV_READ, &p, err, errlen) ||
-            !reg_kernel(g, d, n, "attn_paged", FAM_ATTN, &p, err, errlen)) { ok = false; goto out; }
+            !reg_kernel(g, d, n, "attn_paged", FAM_ATTN, &p, err, errlen) || !reg_kernel(g, d, n, "sample_rows", FAM_SAMPLE, &p, err, errlen)) { ok = false; goto out; }
     }
     if (def_get(d, n, "QW_HIP_MEM")) { // this backend's own measurement helpers
         p = (qw_kparams){0};
@@ -1163,7 +1164,7 @@ static bool fail(qw_batch *b, const char *fmt, ...) {
     return false;
 }
 
-static bool of_attn_family(qw_family f) { return f == FAM_KV_WRITE || f == FAM_KV_READ || f == FAM_ATTN; }
+static bool of_attn_family(qw_family f) { return f == FAM_KV_WRITE || f == FAM_KV_READ || f == FAM_ATTN || f == FAM_SAMPLE; }
 // Binding `index` as a device pointer with at least `need` bytes after its offset; records the use.
 static bool bind_ptr(qw_batch *b, unsigned index, size_t need, bool out, const char *what, void **p) {
     qw_hbuf *h = b->buf[index].h;
@@ -2557,8 +2558,24 @@ static bool tr_attn(qw_batch *b) {
     b->l[b->nl - 1].gy = (unsigned)x.dim / 64, b->l[b->nl - 1].gz = (unsigned)x.q_heads;
     return true;
 }
+// Bindings: 0 logits, 1 parameters, 2 u, 3 ids, 4 probs, 5 ws, 10 qw_sample_geo.
+size_t qw_sample_ws_bytes(const qw_gpu *g, int rows, int vocab) { return !g || rows < 1 || rows > QW_KV_MAX_ROWS || vocab < 1 || vocab > (int)QW_SAMPLE_VOCAB ? 0 : 16; }
+static bool tr_sample(qw_batch *b) {
+    qw_sample_geo x;
+    qwk_sample_args a = {0};
+    if (!bind_bytes(b, QW_ATTN_GEO, &x, sizeof x, "sizes")) return false;
+    if (x.rows < 1 || x.rows > QW_KV_MAX_ROWS || x.vocab < 1 || x.vocab > (int)QW_SAMPLE_VOCAB) return fail(b, "sample_rows: %d rows of %d logits (1 to %d of 1 to %u)", x.rows, x.vocab, QW_KV_MAX_ROWS, QW_SAMPLE_VOCAB);
+    const int stride = x.stride ? x.stride : x.vocab;
+    if (stride < x.vocab) return fail(b, "sample_rows: %d values from row to row of %d logits", stride, x.vocab);
+    const size_t R = (size_t)x.rows;
+    if (!bind_ptr(b, 0, ((R - 1) * (size_t)stride + (size_t)x.vocab) * 4, false, "logits", (void **)&a.logits) || !bind_ptr(b, 1, R * sizeof(qwk_sample_row), false, "parameters", (void **)&a.p) ||
+        !bind_ptr(b, 2, R * 4, false, "u", (void **)&a.u) || !bind_whole(b, 3, R * 4, "ids", (void **)&a.ids) || (b->buf[4].h && !bind_whole(b, 4, R * 4, "probs", (void **)&a.probs))) return false;
+    if ((uintptr_t)a.logits % 4 || (uintptr_t)a.p % 4 || (uintptr_t)a.u % 4 || (uintptr_t)a.ids % 4 || (uintptr_t)a.probs % 4) return fail(b, "sample_rows: every buffer must be 4-byte aligned");
+    a.vocab = (uint32_t)x.vocab, a.stride = (uint32_t)stride;
+    return add_launch(b, "qwk_sample", (unsigned)x.rows, QW_WG_SAMPLE, &a, sizeof a);
+}
 qw_kernel *qw_hip_attn_kernel(qw_batch *b, int which) {
-    static const char *const names[QW_ATTN_CALLS] = {"kv_write", "kv_read", "attn_paged"}, def[] = "#define QW_ATTN 1\n";
+    static const char *const names[QW_ATTN_CALLS] = {"kv_write", "kv_read", "attn_paged", "sample_rows"}, def[] = "#define QW_ATTN 1\n";
     qw_gpu *g = b->g;
     if (!g->attn_k[which] && qw_gpu_compile(g, def, sizeof def - 1, NULL, 0))
         for (int i = 0; i < QW_ATTN_CALLS; i++) g->attn_k[i] = qw_kernel_get(g, names[i]);
@@ -2605,6 +2622,7 @@ void qw_batch_dispatch(qw_batch *b, unsigned gx, unsigned gy, unsigned gz, unsig
     case FAM_KV_WRITE: ok = tr_kv_write(b); break;
     case FAM_KV_READ: ok = tr_kv_read(b); break;
     case FAM_ATTN: ok = tr_attn(b); break;
+    case FAM_SAMPLE: ok = tr_sample(b); break;
     default: ok = tr_mem(b, gx);
     }
     if (ok && b->nl > first) b->l[b->nl - 1].last_of_dispatch = true;

@@ -553,3 +553,5 @@ template <int TYPE> __device__ __forceinline__ void kv_read_body(const qwk_kv_re
 }
 extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_read_f1(qwk_kv_read_args a) { kv_read_body<F16>(a); }
 extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_read_f8(qwk_kv_read_args a) { kv_read_body<Q8>(a); }
+
+#include "qw_sample.hip.h"

@@ -40,6 +40,19 @@ typedef struct {
     uint32_t k_stride, v_stride;
 } qwk_kv_read_args;
 
+typedef struct { float temperature, top_p, min_p; uint32_t top_k; } qwk_sample_row;
+typedef struct {
+    const float *logits;
+    const qwk_sample_row *p;
+    const float *u;
+    uint32_t *ids;
+    float *probs; /* may be NULL */
+    uint32_t vocab, stride;
+} qwk_sample_args;
+#define QW_WG_SAMPLE 1024u
+#define QW_SAMPLE_TILE 4096u      /* tokens of which a row keeps the sum */
+#define QW_SAMPLE_VOCAB (1u << 20) /* at most */
+
 /* What the functions of include/qw_attn.h hand a dispatch beside its buffers, as inline bytes at index QW_ATTN_GEO. */
 #define QW_ATTN_GEO 10u
 typedef struct {
@@ -49,3 +62,4 @@ typedef struct {
     float scale;
     int32_t rot, axes, pairs[3], adjacent;
 } qw_attn_geo;
+typedef struct { int32_t rows, vocab, stride; } qw_sample_geo; /* the same of qw_sample */

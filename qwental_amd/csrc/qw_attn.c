@@ -61,3 +61,12 @@ bool qw_attn(qw_batch *b, const qw_kv *c, const qw_kv_step *s, int q_heads, cons
     bind(b, 6, ws);
     return end(b, &geo);
 }
+bool qw_sample(qw_batch *b, int rows, int vocab, int stride, const qw_at *logits, const qw_at *params, const qw_at *u, const qw_at *ids, const qw_at *probs, const qw_at *ws) {
+    if (!b) return false;
+    const qw_sample_geo geo = {rows, vocab, stride};
+    qw_batch_kernel(b, qw_hip_attn_kernel(b, QW_ATTN_SAMPLE));
+    bind(b, 0, logits), bind(b, 1, params), bind(b, 2, u), bind(b, 3, ids), bind(b, 4, probs), bind(b, 5, ws);
+    qw_batch_bytes(b, QW_ATTN_GEO, &geo, sizeof geo);
+    qw_batch_dispatch(b, 1, 1, 1, 1, 1, 1);
+    return !qw_hip_batch_failed(b);
+}

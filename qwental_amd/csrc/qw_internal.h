@@ -46,7 +46,7 @@ QW_INTERNAL double qw_hip_batch_end_parts(qw_batch *b, double *secs);
 
 /* The kernels of include/qw_attn.h: their code object (qw_attn.c), the kernel of a call (registered with the device at its first use), and whether a
  * dispatch of the batch was refused. */
-enum { QW_ATTN_WRITE, QW_ATTN_READ, QW_ATTN_ATTN, QW_ATTN_CALLS };
+enum { QW_ATTN_WRITE, QW_ATTN_READ, QW_ATTN_ATTN, QW_ATTN_SAMPLE, QW_ATTN_CALLS };
 #define QW_ATTN_MAX_HEADS 256
 #define QW_ATTN_MAX_Q_HEADS 1024
 #define QW_ATTN_MAX_PAGE 65536

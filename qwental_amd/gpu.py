@@ -119,6 +119,7 @@ SYMBOLS = [
 ATTN_SYMBOLS = [
     ("qw_kv_bytes", _sz, [_i, _i, _i, _i, _i]), ("qw_kv_write", _b, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]), ("qw_kv_read", _b, [_vp, _vp, _vp, _vp, _vp]),
     ("qw_attn_ws_bytes", _sz, [_vp, _i]), ("qw_attn", _b, [_vp, _vp, _vp, _i, _vp, _vp, C.c_float, _i, _vp]),
+    ("qw_sample_ws_bytes", _sz, [_vp, _i, _i]), ("qw_sample", _b, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     ("qw_hip_stream_begin", _vp, [_vp, _vp]), ("qw_hip_stream_end", _b, [_vp]), ("qw_hip_buf_view", _b, [_vp, _vp, _sz, _pb]),
 ]
 
