@@ -2531,7 +2531,13 @@ static bool tr_kv_read(qw_batch *b) {
 // Two workgroups a compute unit; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
 static unsigned attn_grid(const qw_gpu *g) { return 2 * (unsigned)g->ncu; }
 static size_t attn_part_bytes(const qw_gpu *g, int dim, unsigned qt) { return (size_t)attn_grid(g) * 2 * 16 * qt * (size_t)dim * 4; }
-size_t qw_attn_ws_bytes(const qw_gpu *g, int dim) { return !g || dim < 64 || dim > 256 || dim % 64 ? 0 : attn_part_bytes(g, dim, 2) + attn_part_bytes(g, 2, 2); }
+size_t qw_attn_ws_bytes(const qw_gpu *g, int dim) { return !g || dim < 64 || dim > 256 || dim % 64 ? 0 : attn_part_bytes(g, dim, 2) + attn_part_bytes(g, 2, 2) + (size_t)attn_grid(g) * 2 * QW_ATTN_PART; }
+// Division by d for dividends below 2^31: with 2^l >= d the least such power, mul = floor(2^(31 + l) / d) + 1 is off by less than 2^l / 2^31 of a step for each of them.
+static qwk_div div_of(uint32_t d) {
+    unsigned l = 0;
+    while ((uint64_t)1 << l < d) l++;
+    return d <= 1 ? (qwk_div){0, 0} : (qwk_div){(uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1};
+}
 static bool tr_attn(qw_batch *b) {
     static const char *const names[2][4][2] = {{{"qwk_attn_f1_d64_q1", "qwk_attn_f1_d64_q2"}, {"qwk_attn_f1_d128_q1", "qwk_attn_f1_d128_q2"}, {"qwk_attn_f1_d192_q1", "qwk_attn_f1_d192_q2"}, {"qwk_attn_f1_d256_q1", "qwk_attn_f1_d256_q2"}},
                                                {{"qwk_attn_f8_d64_q1", "qwk_attn_f8_d64_q2"}, {"qwk_attn_f8_d128_q1", "qwk_attn_f8_d128_q2"}, {"qwk_attn_f8_d192_q1", "qwk_attn_f8_d192_q2"}, {"qwk_attn_f8_d256_q1", "qwk_attn_f8_d256_q2"}}};
@@ -2540,6 +2546,9 @@ static bool tr_attn(qw_batch *b) {
     qw_span cache, q, out, ws;
     if (!kv_bind(b, &x, &a.c, false, &cache)) return false;
     if (x.q_heads < 1 || x.q_heads > QW_ATTN_MAX_Q_HEADS || x.q_heads % x.heads) return fail(b, "attn_paged: %d query heads for %d of keys (a multiple, up to %d)", x.q_heads, x.heads, QW_ATTN_MAX_Q_HEADS);
+    // tiles of all pairs are counted in 32 bits
+    if ((((uint64_t)x.rows * (uint64_t)x.q_heads + 15) / 16 + (uint64_t)x.slots * (uint64_t)x.heads) * ((uint64_t)x.max_pages * (uint64_t)x.page / QW_ATTN_TILE + 2) > INT32_MAX)
+        return fail(b, "attn_paged: %d rows of %d query heads over up to %lld tokens: too many for one call", x.rows, x.q_heads, (long long)x.max_pages * x.page);
     if (x.window < 0 || !(x.scale >= 0) || x.scale > 1e30f) return fail(b, "attn_paged: window %d, scale %g", x.window, (double)x.scale);
     if (!kv_rows(b, 4, false, &x, x.q_heads, x.stride[0], "q", (uint16_t **)&a.q, &a.q_stride, &q) || !kv_rows(b, 5, true, &x, x.q_heads, x.stride[1], "out", &a.out, &a.out_stride, &out)) return false;
     const size_t need = qw_attn_ws_bytes(b->g, x.dim);
@@ -2553,9 +2562,11 @@ static bool tr_attn(qw_batch *b) {
     // rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode
     const unsigned qt = cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
     a.ml = a.part + attn_part_bytes(b->g, x.dim, 2) / 4;
+    a.parts = a.ml + attn_part_bytes(b->g, 2, 2) / 4;
+    a.by_group = div_of(a.group);
     if (!add_launch(b, names[x.type == 8][x.dim / 64 - 1][qt - 1], a.grid, QW_WG_ATTN, &a, sizeof a)) return false;
-    if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", (unsigned)x.rows, QW_WG_JOIN, &a, sizeof a)) return false;
-    b->l[b->nl - 1].gy = (unsigned)x.dim / 64, b->l[b->nl - 1].gz = (unsigned)x.q_heads;
+    if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", a.grid, QW_WG_JOIN, &a, sizeof a)) return false;
+    b->l[b->nl - 1].gy = 2; // of the pair that a workgroup went on with, and of the one that it began
     return true;
 }
 // Bindings: 0 logits, 1 parameters, 2 u, 3 ids, 4 probs, 5 ws, 10 qw_sample_geo.

@@ -11,6 +11,8 @@ typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
+typedef unsigned long long u64;
+
 enum { F16 = 1, Q8 = 8 };
 
 // ---------------------------------------------------------------- attention
@@ -26,13 +28,17 @@ enum { F16 = 1, Q8 = 8 };
 
 struct Slot { int n, len, first; }; // rows, tokens, first row
 
+// first, len and table are nobody's output: read as constants, with a uniform index through the scalar cache, whose loads do not wait for the streams'.
+typedef const uint32_t __attribute__((address_space(4))) *const_words;
+__device__ __forceinline__ const_words words(const uint32_t *p) { return (const_words)(uintptr_t)p; }
+
 __device__ __forceinline__ Slot slot_of(const qwk_kv &c, uint32_t i) {
-    const uint32_t a = c.first[i], b = c.first[i + 1], l = c.len[i];
-    const uint64_t room = (uint64_t)c.max_pages << c.page_log2;
+    uint32_t a = words(c.first)[i], b = words(c.first)[i + 1], l = words(c.len)[i];
+    const uint32_t room = c.max_pages << c.page_log2; // (up to 2^30)
     Slot s;
     s.first = (int)a;
-    s.n = a <= b && b <= c.rows ? (int)(b - a) : 0; // what is no row of the step is not touched
-    s.len = (int)(l < room ? l : room);
+    s.n = (a <= b) & (b <= c.rows) ? (int)(b - a) : 0; // what is no row of the step is not touched
+    s.len = (int)min(l, room);
     return s;
 }
 // The slot of a row, by a whole wave in one round trip; false: it belongs to none.
@@ -40,51 +46,71 @@ __device__ __forceinline__ bool slot_find(const qwk_kv &c, uint32_t row, uint32_
     i = 0;
     for (uint32_t at = 0; at < c.slots; at += 64) {
         const uint32_t k = at + (threadIdx.x & 63);
-        i += (uint32_t)__popcll(__ballot(k < c.slots && c.first[k + 1] <= row));
+        i += (uint32_t)__popcll(__ballot(k < c.slots && words(c.first)[k + 1] <= row));
     }
     if (i >= c.slots) return false;
     s = slot_of(c, i);
     return (int)row >= s.first && (int)row < s.first + s.n;
 }
+__device__ __forceinline__ int by(qwk_div d, int x) { return d.mul ? (int)(__umulhi((uint32_t)x, d.mul) >> d.shift) : x; } // x / d, 0 <= x < 2^31
+
 struct Range { int t0, cnt; }; // a block's first tile, and how many (at least one: an empty one still gives its rows their zeros)
-template <int QT> __device__ __forceinline__ Range block_range(const Slot &s, int b, int group, int window) {
-    const int M = s.n * group, j0 = b * 16 * QT / group, m1 = min((b + 1) * 16 * QT, M) - 1, j1 = m1 / group;
-    const int hi = s.len - s.n + j1 + 1, lo = window ? max(0, s.len - s.n + j0 - window + 1) : 0;
+template <int QT> __device__ __forceinline__ Range block_range(const Slot &s, int b, const qwk_attn_args &a) {
+    const int M = s.n * (int)a.group, j0 = by(a.by_group, b * 16 * QT), j1 = by(a.by_group, min((b + 1) * 16 * QT, M) - 1);
+    const int hi = s.len - s.n + j1 + 1, lo = a.window ? max(0, s.len - s.n + j0 - (int)a.window + 1) : 0;
     Range r;
     r.t0 = hi > 0 ? lo / (int)QW_ATTN_TILE : 0;
     r.cnt = hi > 0 ? max(1, (hi + (int)QW_ATTN_TILE - 1) / (int)QW_ATTN_TILE - r.t0) : 1;
     return r;
 }
-template <int QT> __device__ __forceinline__ int blocks_of(const Slot &s, int group) { return (s.n * group + 16 * QT - 1) / (16 * QT); }
+template <int QT> __device__ __forceinline__ int blocks_of(const Slot &s, const qwk_attn_args &a) { return (s.n * (int)a.group + 16 * QT - 1) / (16 * QT); }
 
-struct Plan { // LDS
-    uint64_t end[QW_KV_SLOTS_MAX]; // tiles of the slots up to and with this one
-    uint64_t wave[4];
-};
-// Tiles of all slots, by the whole workgroup; returns the total.
-template <int QT> __device__ uint64_t make_plan(Plan &p, const qwk_kv &c, int group, int window) {
-    const uint32_t i = threadIdx.x, lane = i & 63;
-    uint64_t t = 0;
-    if (i < c.slots) {
-        const Slot s = slot_of(c, i);
-        const int nb = blocks_of<QT>(s, group);
-        for (int b = 0; b < nb; b++) t += (uint64_t)block_range<QT>(s, b, group, window).cnt;
-        t *= c.heads;
-    }
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(t, d);
-        if (lane >= (uint32_t)d) t += o;
-    }
-    if (lane == 63) p.wave[i >> 6] = t;
-    __syncthreads();
-    for (uint32_t w = 0; w < (i >> 6); w++) t += p.wave[w];
-    if (i < QW_KV_SLOTS_MAX) p.end[i] = t;
-    __syncthreads();
-    return p.end[QW_KV_SLOTS_MAX - 1];
+// Tiles of all slots, a lane a slot. Every wave makes it and writes it down for itself (all the same, where it is the same LDS): no barrier.
+struct Plan { uint32_t each[QW_KV_SLOTS_MAX], end[QW_KV_SLOTS_MAX]; }; // tiles of one of the slot's heads; of all slots up to and with this one
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) { // sums over the lanes up to and with this one
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false); // row_shr:1, 2, 4, 8
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false); // row_bcast:15, 31
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+    return x;
 }
-// Shares: workgroup w of g takes the tiles [w T / g, (w + 1) T / g). No more workgroups than there are four tiles for (one a wave).
-__device__ __forceinline__ uint64_t shares_of(uint64_t T, uint32_t grid) { return min((uint64_t)grid, (T + 3) / 4); }
-__device__ __forceinline__ uint32_t owner_of(uint64_t x, uint64_t T, uint64_t g) { return (uint32_t)(((x + 1) * g - 1) / T); }
+template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, uint32_t &pairs) { // returns the tiles of all
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t T = 0;
+    pairs = 0;
+#pragma unroll 1
+    for (uint32_t k = 0; k < a.c.slots; k += 64) {
+        const uint32_t i = k + lane;
+        uint32_t each = 0;
+        Slot s = slot_of(a.c, min(i, a.c.slots - 1));
+        asm volatile("" : "+v"(s.n), "+v"(s.len)); // (all three loads at once, not the length's behind a branch on the others)
+        const int nb = i < a.c.slots ? blocks_of<QT>(s, a) : 0;
+#pragma unroll 1
+        for (int b = 0; b < nb; b++) each += (uint32_t)block_range<QT>(s, b, a).cnt;
+        const uint32_t end = T + wave_scan(each * a.c.heads);
+        p.each[i] = each, p.end[i] = end;
+        T = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+        pairs += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)nb), 63);
+    }
+    pairs *= a.c.heads;
+    return T;
+}
+// Shares: workgroup w of g takes the next T / g tiles, the first T % g of them one more.
+struct Shares {
+    uint32_t g, base, more;
+    // As many workgroups as there are four tiles for, one a wave, or pairs: behind its first pair's end a workgroup starts once more (3 us; a slot of one token and four heads: one
+    // workgroup for all of them 15.9 us, four 6)
+    __device__ __forceinline__ Shares(uint32_t T, uint32_t pairs, uint32_t grid) : g(min(grid, max((T + 3) / 4, pairs))), base(0), more(0) {
+        if (g) base = T / g, more = T - base * g;
+    }
+    __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * base + min(w, more); }
+    __device__ __forceinline__ uint32_t owner(uint32_t x) const {
+        const uint32_t big = more * (base + 1);
+        return x < big ? x / (base + 1) : more + (x - big) / base;
+    }
+};
 
 // Four codes -> binary16, exactly: 0x64 in front of a byte b is 1024 + b, and b is the code + 128.
 __device__ __forceinline__ half4_t codes(uint32_t w) {
@@ -95,23 +121,50 @@ __device__ __forceinline__ half4_t codes(uint32_t w) {
     return half4_t{lo.x, lo.y, hi.x, hi.y};
 }
 
-template <int TYPE, int D> struct UnitData; // a lane's share of U units: keys or values, and their scales
+template <int TYPE, int D> struct UnitData; // a lane's share of a unit: keys or values, and their scales
 template <int D> struct UnitData<F16, D> {
     uint4_t x[D / 32];
-    __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t lane) {
-        const uint8_t *p = u + (values ? 32 * D : 0) + lane * 16;
+    __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t at, uint32_t) {
+        const uint8_t *p = u + (values ? 32 * D : 0) + at;
 #pragma unroll
         for (int c = 0; c < D / 32; c++) x[c] = *(const uint4_t *)(p + c * 1024);
     }
+    // Of values: zeros in place of the lane's tokens that `keep` (two halves a word) has no bits for; which of the four tokens hold what is not finite (bits of 0x7c00 in each half)
+    __device__ __forceinline__ void mask(uint2_t keep) {
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) x[c] &= uint4_t{keep.x, keep.y, keep.x, keep.y};
+    }
+    __device__ __forceinline__ uint2_t odd() const {
+        uint2_t o = {0, 0};
+        const auto full = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }; // (neither half carries into the other: its sign is masked)
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) o |= uint2_t{full(x[c].x) | full(x[c].z), full(x[c].y) | full(x[c].w)};
+        return o;
+    }
+    static __device__ __forceinline__ float value(const uint8_t *u, uint32_t t, uint32_t v) { return (float)*(const _Float16 *)(u + 32 * D + (v / 32 * 512 + t / 4 * 128 + v % 32 * 4 + t % 4) * 2); }
 };
 template <int D> struct UnitData<Q8, D> {
     uint4_t x[D / 64], s[D / 64];
-    __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t lane) {
+    __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t at, uint32_t scale_at) {
         const uint8_t *p = u + (values ? 17 * D : 0);
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) x[c] = *(const uint4_t *)(p + c * 1024 + lane * 16);
+        for (int c = 0; c < D / 64; c++) x[c] = *(const uint4_t *)(p + c * 1024 + at);
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) s[c] = *(const uint4_t *)(p + 16 * D + (lane >> 4) * (D / 4) + c * 16);
+        for (int c = 0; c < D / 64; c++) s[c] = *(const uint4_t *)(p + 16 * D + scale_at + c * 16);
+    }
+    __device__ __forceinline__ void mask(uint2_t keep) { // (codes are finite: it is the scales that are not)
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) s[c] &= uint4_t{keep.x, keep.y, keep.x, keep.y};
+    }
+    __device__ __forceinline__ uint2_t odd() const {
+        uint2_t o = {0, 0};
+        const auto full = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) o |= uint2_t{full(s[c].x) | full(s[c].z), full(s[c].y) | full(s[c].w)};
+        return o;
+    }
+    static __device__ __forceinline__ float value(const uint8_t *u, uint32_t t, uint32_t v) {
+        return (float)*(const int8_t *)(u + 17 * D + v / 64 * 1024 + t / 4 * 256 + v % 32 / 2 * 16 + v / 32 % 2 * 8 + v % 2 * 4 + t % 4) * (float)*(const _Float16 *)(u + 33 * D + (t / 4 * (D / 32) + v / 32) * 8 + t % 4 * 2);
     }
     __device__ __forceinline__ half4_t scales(int b) const { // of block b, tokens 4 (lane >> 4) + i
         return __builtin_bit_cast(half4_t, b & 1 ? uint2_t{s[b / 2].z, s[b / 2].w} : uint2_t{s[b / 2].x, s[b / 2].y});
@@ -120,17 +173,13 @@ template <int D> struct UnitData<Q8, D> {
 
 template <int TYPE, int D, int QT, int U> struct Attn {
     const qwk_attn_args &a;
-    const uint32_t lane, wave;
+    const uint32_t lane;
     half8_t q[QT][D / 32];
     float4_t acc[QT][D / 32][2]; // result: value 32 b + 8 (lane >> 4) + 2 i + c of query lane & 15
     float m[QT], l[QT];          // reference (log2) and this lane's part of the sum
-    int hi[QT], lo[QT], tok[QT]; // tokens [lo, hi) that the lane's query sees, and which of the slot's rows it is
+    int hi[QT], lo[QT];          // tokens [lo, hi) that the lane's query sees
     UnitData<TYPE, D> K[U], V[U];
 
-    __device__ __forceinline__ void load(bool values, const uint8_t *const *u) {
-#pragma unroll
-        for (int i = 0; i < U; i++) (values ? V : K)[i].load(u[i], values, lane);
-    }
     __device__ __forceinline__ float4_t scores(int t, int i) {
         float4_t s = {0, 0, 0, 0};
         if constexpr (TYPE == F16) {
@@ -150,158 +199,167 @@ template <int TYPE, int D, int QT, int U> struct Attn {
         }
         return s;
     }
-    // Weights in two parts, binary16 each: together they hold 22 bits, so that the result is as exact as its own rounding. The largest weight is 2^TOP, not 1, so that the
+    // Weights in two parts, binary16 each: together they hold 21 bits, so that the result is as exact as its own rounding. The largest weight is 2^TOP, not 1, so that the
     // small ones do not end at binary16's 2^-24: many tokens of 2^-25 of the largest's weight count for something together. (Q8_0: a weight is multiplied by a scale of up to 516.)
     static constexpr float TOP = TYPE == F16 ? 14.f : 6.f;
     __device__ __forceinline__ static void split(const float4_t &p, half4_t &h, half4_t &r) {
+        const half2_t h0 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(p[0], p[1])), h1 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(p[2], p[3]));
+        float d[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) h[j] = (_Float16)p[j], r[j] = (_Float16)(p[j] - (float)h[j]);
+        for (int j = 0; j < 4; j++) d[j] = __builtin_fmaf((float)(j < 2 ? h0 : h1)[j & 1], -1.f, p[j]);
+        const half2_t r0 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(d[0], d[1])), r1 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(d[2], d[3]));
+        h = half4_t{h0.x, h0.y, h1.x, h1.y}, r = half4_t{r0.x, r0.y, r1.x, r1.y};
     }
     __device__ __forceinline__ half4_t values(int i, int b, int c) const {
         if constexpr (TYPE == F16) return __builtin_bit_cast(half4_t, c ? uint2_t{V[i].x[b].z, V[i].x[b].w} : uint2_t{V[i].x[b].x, V[i].x[b].y});
         else return codes(V[i].x[b / 2][(b & 1) * 2 + c]);
     }
+    __device__ __forceinline__ bool hidden(int t, int key, uint32_t bad, int i) const { return key >= hi[t] || key < lo[t] || (bad >> i & 1); }
     // key0: first token of the step's first unit; bad: units without a page; edge: some query does not see all of the step's tokens
     __device__ __forceinline__ void softmax(int key0, uint32_t bad, bool edge, float4_t (&p)[QT][U]) {
         const float neg = -__builtin_inff();
+        if (edge)
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int i = 0; i < U; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (hidden(t, key0 + i * 16 + (int)(lane >> 4) * 4 + j, bad, i)) p[t][i][j] = neg;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-#pragma unroll
-            for (int i = 0; i < U; i++) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    p[t][i][j] *= a.scale;
-                    if (edge) {
-                        const int key = key0 + i * 16 + (int)(lane >> 4) * 4 + j;
-                        if (key >= hi[t] || key < lo[t] || (bad >> i & 1)) p[t][i][j] = neg;
-                    }
-                }
-            }
             float top = neg;
 #pragma unroll
             for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) top = fmaxf(top, p[t][i][j]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m[t])) {
+            top *= a.scale;
+            if (__any(top > m[t])) { // (as a rule in a wave's first steps only)
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
                 const float now = fmaxf(m[t], top), f = m[t] == neg ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
                 m[t] = now;
                 l[t] *= f;
 #pragma unroll
                 for (int b = 0; b < D / 32; b++) acc[t][b][0] *= f, acc[t][b][1] *= f;
             }
-            const float ref = m[t] == neg ? 0.f : m[t] - TOP;
+            const float ref = m[t] == neg ? 0.f : TOP - m[t];
 #pragma unroll
             for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    p[t][i][j] = __builtin_amdgcn_exp2f(p[t][i][j] - ref);
+                    p[t][i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i][j], a.scale, ref));
                     l[t] += p[t][i][j];
                 }
         }
     }
-    __device__ __forceinline__ void weigh(int key0, uint32_t bad, bool edge, const float4_t (&p)[QT][U]) {
+    __device__ __forceinline__ void weigh(const float4_t (&p)[QT][U]) {
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const int key = key0 + i * 16 + (int)(lane >> 4) * 4;
-            if constexpr (TYPE == F16) {
-                half4_t h[QT], r[QT];
+            half4_t h[QT], r[QT];
+            if constexpr (TYPE == F16)
 #pragma unroll
                 for (int t = 0; t < QT; t++) split(p[t][i], h[t], r[t]);
-                if (!edge) {
+#pragma unroll
+            for (int b = 0; b < D / 32; b++) {
+                const half4_t v0 = values(i, b, 0), v1 = values(i, b, 1);
+                if constexpr (TYPE == Q8) {
+                    const half4_t f = V[i].scales(b); // a token's scale belongs to its weight
+#pragma unroll
+                    for (int t = 0; t < QT; t++) {
+                        float4_t w;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) w[k] = p[t][i][k] * (float)f[k];
+                        split(w, h[t], r[t]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, h[t], acc[t][b][0], 0, 0, 0);
+                    acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, h[t], acc[t][b][1], 0, 0, 0);
+                    acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, r[t], acc[t][b][0], 0, 0, 0);
+                    acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, r[t], acc[t][b][1], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // A token that some queries do not see may hold anything, infinities and NaN too, and 0 times those is not 0. So at the edges: values of tokens that no query of the
+    // block sees become zeros; a token that some see and that holds what is not finite is taken out of the product too, and comes back by itself
+    // (odd_tokens) for those that see it. Returns such tokens of unit i as bits.
+    __device__ __forceinline__ uint32_t clean(int i, int key0, uint32_t bad, int all_lo, int all_hi) {
+        const int key = key0 + i * 16 + (int)(lane >> 4) * 4;
+        const auto unseen = [&](int k) { return key + k >= all_hi || key + k < all_lo || (bad >> i & 1); };
+        V[i].mask(uint2_t{(unseen(0) ? 0u : 0xffffu) | (unseen(1) ? 0u : 0xffff0000u), (unseen(2) ? 0u : 0xffffu) | (unseen(3) ? 0u : 0xffff0000u)});
+        const uint2_t o = V[i].odd();
+        if (!__any((o.x | o.y) != 0)) return 0;
+        uint32_t tokens = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const u64 at = __ballot((o[k / 2] >> (k & 1 ? 31 : 15) & 1) != 0);
+#pragma unroll
+            for (int g = 0; g < 4; g++) tokens |= (at >> g * 16 & 0xffff) ? 1u << (g * 4 + k) : 0;
+        }
+        const uint32_t mine = tokens >> (lane >> 4) * 4;
+        V[i].mask(uint2_t{(mine & 1 ? 0u : 0xffffu) | (mine & 2 ? 0u : 0xffff0000u), (mine & 4 ? 0u : 0xffffu) | (mine & 8 ? 0u : 0xffff0000u)});
+        return tokens;
+    }
+    __device__ __forceinline__ void odd_tokens(int i, uint32_t tokens, const uint8_t *u, int key0, uint32_t bad, const float4_t (&p)[QT][U]) {
+#pragma unroll 1
+        for (; tokens; tokens &= tokens - 1) {
+            const int k = __builtin_ctz(tokens);
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                const float4_t x = p[t][i];
+                const float w = __shfl(k & 2 ? (k & 1 ? x[3] : x[2]) : (k & 1 ? x[1] : x[0]), (int)(lane & 15) + (k >> 2) * 16);
+                if (!hidden(t, key0 + i * 16 + k, bad, i))
 #pragma unroll
                     for (int b = 0; b < D / 32; b++)
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const half4_t v = values(i, b, c);
-#pragma unroll
-                            for (int t = 0; t < QT; t++) {
-                                acc[t][b][c] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, h[t], acc[t][b][c], 0, 0, 0);
-                                acc[t][b][c] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, r[t], acc[t][b][c], 0, 0, 0);
-                            }
-                        }
-                    continue;
-                }
-                // A token that some queries do not see may hold anything, infinities and NaN too, and 0 times those is not 0: the slot's rows
-                // one after the other, each with the values that it sees and zeros in the others' place, its own columns kept
-#pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    const int j0 = __builtin_amdgcn_readfirstlane(tok[t]), j1 = __builtin_amdgcn_readlane(tok[t], 15);
-                    for (int j = j0; j <= j1; j++) {
-                        const int d = j - j0;
-                        const int hj = __builtin_amdgcn_readfirstlane(hi[t]) + d, lj = a.window ? max(0, hj - (int)a.window) : 0;
-                        const bool mine = tok[t] == j;
-#pragma unroll
-                        for (int b = 0; b < D / 32; b++)
-#pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                half4_t v = values(i, b, c);
-#pragma unroll
-                                for (int k = 0; k < 4; k++)
-                                    if (key + k >= hj || key + k < lj || (bad >> i & 1)) v[k] = (_Float16)0.f;
-                                float4_t s = __builtin_amdgcn_mfma_f32_16x16x16f16(v, h[t], acc[t][b][c], 0, 0, 0);
-                                s = __builtin_amdgcn_mfma_f32_16x16x16f16(v, r[t], s, 0, 0, 0);
-                                if (mine) acc[t][b][c] = s;
-                            }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int b = 0; b < D / 32; b++) {
-                    const half4_t f = V[i].scales(b);
-                    const half4_t v0 = values(i, b, 0), v1 = values(i, b, 1);
-#pragma unroll
-                    for (int t = 0; t < QT; t++) {
-                        float4_t w; // a token's scale belongs to its weight: codes are finite, so what is not seen is 0 whatever its scale
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            w[k] = p[t][i][k] * (float)f[k];
-                            if (edge && (key + k >= hi[t] || key + k < lo[t] || (bad >> i & 1))) w[k] = 0.f;
-                        }
-                        half4_t h, r;
-                        split(w, h, r);
-                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, h, acc[t][b][0], 0, 0, 0);
-                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, r, acc[t][b][0], 0, 0, 0);
-                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, h, acc[t][b][1], 0, 0, 0);
-                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, r, acc[t][b][1], 0, 0, 0);
-                    }
-                }
+                        for (int j = 0; j < 8; j++) acc[t][b][j & 1][j >> 1] += w * UnitData<TYPE, D>::value(u, (uint32_t)k, (uint32_t)b * 32 + (lane >> 4) * 8 + (uint32_t)j);
             }
         }
     }
 };
 
+// What a workgroup leaves for the join, twice: of the pair that it went on with, and of the one that it began and did not end.
+struct Part {
+    uint32_t rows, row0, m0, head, w0, w1; // rows 0: none; the pair's block: first row of the slot, first row x query head, and the workgroups that share it
+    uint32_t pad[2];
+};
+static_assert(sizeof(Part) == QW_ATTN_PART, "");
+
 template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
-    constexpr int U = D <= 128 ? 2 : 1, W = QW_WG_ATTN / 64, LD = D + 4; // U: units a wave has in hand; a tile is two
-    __shared__ Plan plan;
-    __shared__ float so[W][16][LD], sm[W][16], sl[W][16];
+    constexpr int U = D <= 128 ? 2 : 1, W = QW_WG_ATTN / 64, LD = D + 4, STEPS = 2 / U; // U: units a wave has in hand; a tile is two
+    __shared__ float4_t so[W][16][LD / 4];
+    __shared__ float sm[W][16], sl[W][16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const qwk_kv &c = a.c;
     const int group = (int)a.group, window = (int)a.window;
-    const uint64_t T = make_plan<QT>(plan, c, group, window), g = shares_of(T, a.grid);
-    if (blockIdx.x >= g) return;
-    uint64_t x = blockIdx.x * T / g;
-    const uint64_t end = (blockIdx.x + 1) * T / g;
+    Part *parts = (Part *)a.parts + blockIdx.x * 2;
+    __shared__ Plan plan;
+    uint32_t pairs;
+    const uint32_t T = make_plan<QT>(plan, a, pairs);
+    const Shares sh(T, pairs, a.grid);
+    if (threadIdx.x < 2) parts[threadIdx.x].rows = 0;
+    if (blockIdx.x >= sh.g) return;
+    uint32_t x = sh.start(blockIdx.x);
+    const uint32_t end = sh.start(blockIdx.x + 1);
     while (x < end) {
         uint32_t i = 0; // the slot that tile x belongs to
-        for (uint32_t step = QW_KV_SLOTS_MAX / 2; step; step >>= 1)
-            if (plan.end[i + step - 1] <= x) i += step;
+        for (uint32_t k = 0; k < c.slots; k += 64) i += (uint32_t)__popcll(__ballot(plan.end[k + lane] <= x));
         const Slot s = slot_of(c, i);
-        const uint64_t base = i ? plan.end[i - 1] : 0, per_head = (plan.end[i] - base) / c.heads;
-        const uint32_t head = (uint32_t)((x - base) / per_head);
-        uint64_t rest = x - base - head * per_head;
-        int blk = 0;
-        Range r = block_range<QT>(s, 0, group, window);
-        while (rest >= (uint64_t)r.cnt) rest -= (uint64_t)r.cnt, r = block_range<QT>(s, ++blk, group, window);
-        const int from = (int)rest, to = (int)min((uint64_t)r.cnt, rest + (end - x));
+        const uint32_t each = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan.each[i]), base = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan.end[i]) - each * c.heads;
+        const uint32_t head = (x - base) / each;
+        int from = (int)(x - base - head * each), blk = 0;
+        Range r = block_range<QT>(s, 0, a);
+        while (from >= r.cnt) from -= r.cnt, r = block_range<QT>(s, ++blk, a);
+        const int to = min(r.cnt, from + (int)(end - x));
         const int M = s.n * group, m0 = blk * 16 * QT;
 
-        Attn<TYPE, D, QT, U> A{a, lane, wave};
+        Attn<TYPE, D, QT, U> A{a, lane};
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-            const int row = min(m0 + t * 16 + (int)(lane & 15), M - 1), j = row / group;
-            A.tok[t] = j;
+            const int row = min(m0 + t * 16 + (int)(lane & 15), M - 1), j = by(a.by_group, row);
             A.hi[t] = s.len - s.n + j + 1;
             A.lo[t] = window ? max(0, A.hi[t] - window) : 0;
             A.m[t] = -__builtin_inff(), A.l[t] = 0;
@@ -311,55 +369,95 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
 #pragma unroll
             for (int b = 0; b < D / 32; b++) A.acc[t][b][0] = A.acc[t][b][1] = float4_t{0, 0, 0, 0};
         }
-        // what every query of the block sees: [see_lo, see_hi); what some query sees ends at all_hi
-        const int jl = m0 / group, jh = (min(m0 + 16 * QT, M) - 1) / group;
-        const int see_hi = s.len - s.n + jl + 1, see_lo = window ? max(0, s.len - s.n + jh + 1 - window) : 0;
+        // a step's units: where they lie, and which of them have no page
         const int pu = (int)c.page_log2 - 4; // log2 of a page's units
-        const uint32_t *table = c.table + (size_t)i * c.max_pages;
+        const const_words table = words(c.table) + (size_t)i * c.max_pages;
         const size_t in_page = (size_t)head << pu;
-        constexpr int STEPS = 2 / U; // of a tile
-        for (int t = from + (int)wave; t < to; t += W)
-            for (int h = 0; h < STEPS; h++) {
-                const int key0 = (r.t0 + t) * (int)QW_ATTN_TILE + h * 16 * U;
-                const uint8_t *u[U];
-                uint32_t bad = 0;
+        const uint8_t *u[U];
+        uint32_t bad;
+        const auto find = [&](int key0) {
+            bad = 0;
 #pragma unroll
-                for (int k = 0; k < U; k++) {
-                    const uint32_t un = (uint32_t)(key0 >> 4) + k, at = un >> pu;
-                    uint32_t page = at < c.max_pages ? table[at] : 0xffffffffu;
-                    if (page >= c.pages) bad |= 1u << k, page = 0;
-                    u[k] = c.cache + page * c.page_bytes + (in_page + (un & ((1u << pu) - 1))) * c.unit;
-                }
-                A.load(false, u);
-                A.load(true, u);
-                const bool edge = bad || key0 < see_lo || key0 + 16 * U > see_hi;
-                float4_t p[QT][U];
-#pragma unroll
-                for (int q = 0; q < QT; q++)
-#pragma unroll
-                    for (int k = 0; k < U; k++) p[q][k] = A.scores(q, k);
-                A.softmax(key0, bad, edge, p);
-                A.weigh(key0, bad, edge, p);
+            for (int k = 0; k < U; k++) {
+                const uint32_t un = (uint32_t)(key0 >> 4) + k, at = un >> pu;
+                uint32_t page = at < c.max_pages ? table[at] : 0xffffffffu;
+                if (page >= c.pages) bad |= 1u << k, page = 0;
+                u[k] = c.cache + page * c.page_bytes + (in_page + (un & ((1u << pu) - 1))) * c.unit;
             }
+        };
+        const int steps = max(0, (to - from - (int)wave + W - 1) / W) * STEPS;
+        const auto key_of_step = [&](int n) { return (r.t0 + from + (int)wave + n / STEPS * W) * (int)QW_ATTN_TILE + n % STEPS * 16 * U; };
+        // (The queries are asked for before the first step's units: behind them they would be waited for with everything, every step, as the loop's wait has to do for its first.)
+        __builtin_amdgcn_sched_barrier(0);
+        int key0 = key_of_step(0);
+        const uint32_t at = lane * 16, scale_at = (lane >> 4) * (D / 4);
+        find(key0);
+#pragma unroll
+        for (int k = 0; k < U; k++) A.K[k].load(u[k], false, steps ? at : 0, steps ? scale_at : 0);
+#pragma unroll
+        for (int k = 0; k < U; k++) A.V[k].load(u[k], true, steps ? at : 0, steps ? scale_at : 0);
+        // what every query of the block sees: [see_lo, see_hi), and what any of them does: [all_lo, all_hi)
+        const int see_hi = s.len - s.n + by(a.by_group, m0) + 1, all_hi = s.len - s.n + by(a.by_group, min(m0 + 16 * QT, M) - 1) + 1;
+        const int see_lo = window ? max(0, all_hi - window) : 0, all_lo = window ? max(0, see_hi - window) : 0;
+        for (int n = 0; n < steps; n++) {
+            const int key = key0;
+            const uint32_t none = bad;
+            const uint8_t *now[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) now[k] = u[k];
+            const bool edge = none || key < see_lo || key + 16 * U > see_hi;
+            // The next step's loads go out as registers come free: keys behind the scores, values behind the second product. There is one set a step, the last step's too
+            // (16 bytes of its own units, which it does not use): the compiler then knows how many are in flight.
+            const bool more = n + 1 < steps;
+            key0 = more ? key_of_step(n + 1) : key;
+            find(key0);
+            const uint32_t nat = more ? at : 0, nscale = more ? scale_at : 0;
+            float4_t p[QT][U];
+#pragma unroll
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int t = 0; t < QT; t++) p[t][k] = A.scores(t, k);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < U; k++) A.K[k].load(u[k], false, nat, nscale);
+            __builtin_amdgcn_sched_barrier(0);
+            A.softmax(key, none, edge, p);
+            uint32_t odd = 0;
+            if (edge)
+#pragma unroll
+                for (int k = 0; k < U; k++) odd |= A.clean(k, key, none, all_lo, all_hi) << 16 * k;
+            A.weigh(p);
+            if (odd)
+#pragma unroll
+                for (int k = 0; k < U; k++) A.odd_tokens(k, odd >> 16 * k & 0xffff, now[k], key, none, p);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < U; k++) A.V[k].load(u[k], true, nat, nscale);
+        }
         // the waves' results together, in the waves' order
         const bool whole = from == 0 && to == r.cnt;
-        const size_t slot = (size_t)blockIdx.x * 2 + (from == 0);
+        const uint32_t which = from == 0, slot = blockIdx.x * 2 + which;
+        if (!whole && threadIdx.x == 0) {
+            const uint32_t x0 = x - (uint32_t)from;
+            Part p = {(uint32_t)min(16 * QT, M - m0), (uint32_t)s.first, (uint32_t)m0, head, sh.owner(x0), sh.owner(x0 + (uint32_t)r.cnt - 1), {0, 0}};
+            parts[which] = p;
+        }
 #pragma unroll
         for (int t = 0; t < QT; t++) {
+            if (m0 + t * 16 >= M) break;
             float l = A.l[t];
             l += __shfl_xor(l, 16);
             l += __shfl_xor(l, 32);
             __syncthreads();
             if (lane < 16) sm[wave][lane] = A.m[t], sl[wave][lane] = l;
 #pragma unroll
-            for (int b = 0; b < D / 32; b++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float *o = &so[wave][lane & 15][b * 32 + (lane >> 4) * 8 + 2 * k];
-                    o[0] = A.acc[t][b][0][k], o[1] = A.acc[t][b][1][k];
-                }
+            for (int b = 0; b < D / 32; b++) {
+                const float4_t u0 = A.acc[t][b][0], u1 = A.acc[t][b][1];
+                float4_t *o = &so[wave][lane & 15][b * 8 + (lane >> 4) * 2];
+                o[0] = float4_t{u0[0], u1[0], u0[1], u1[1]}, o[1] = float4_t{u0[2], u1[2], u0[3], u1[3]};
+            }
             __syncthreads();
-            const int row = threadIdx.x / 16, mr = m0 + t * 16 + row, v0 = (int)(threadIdx.x % 16) * (D / 16);
+            const int row = threadIdx.x / 16, mr = m0 + t * 16 + row;
             if (mr < M) {
                 float top = -__builtin_inff(), sum = 0, f[W];
                 for (int w = 0; w < W; w++) top = fmaxf(top, sm[w][row]);
@@ -367,69 +465,72 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
                     f[w] = sm[w][row] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm[w][row] - top);
                     sum += sl[w][row] * f[w];
                 }
-                const int j = mr / group;
-                uint16_t *out = a.out + (size_t)(s.first + j) * a.out_stride + ((size_t)head * group + (mr - j * group)) * D + v0;
-                float *part = a.part + (slot * 16 * QT + t * 16 + row) * D + v0;
-                if (!whole && v0 == 0) a.ml[(slot * 16 * QT + t * 16 + row) * 2] = top, a.ml[(slot * 16 * QT + t * 16 + row) * 2 + 1] = sum;
+                const int j = by(a.by_group, mr);
+                uint16_t *out = a.out + (size_t)(s.first + j) * a.out_stride + ((size_t)head * group + (mr - j * group)) * D;
+                const size_t left = (size_t)slot * 16 * QT + t * 16 + row;
+                if (!whole && threadIdx.x % 16 == 0) a.ml[left * 2] = top, a.ml[left * 2 + 1] = sum;
                 const float inv = top == -__builtin_inff() ? 0.f : 1.f / sum; // a row that sees nothing: zeros
-                for (int v = 0; v < D / 16; v++) {
-                    float o = 0;
-                    for (int w = 0; w < W; w++) o += so[w][row][v0 + v] * f[w];
-                    if (whole) out[v] = __builtin_bit_cast(uint16_t, (_Float16)(top == -__builtin_inff() ? 0.f : o * inv));
-                    else part[v] = o;
+#pragma unroll
+                for (int v = 0; v < D / 64; v++) {
+                    const int at4 = v * 16 + (int)(threadIdx.x % 16);
+                    float4_t o = {0, 0, 0, 0};
+                    for (int w = 0; w < W; w++) o += so[w][row][at4] * f[w];
+                    if (whole) {
+                        half4_t h;
+                        for (int k = 0; k < 4; k++) h[k] = (_Float16)(top == -__builtin_inff() ? 0.f : o[k] * inv);
+                        *(half4_t *)(out + at4 * 4) = h;
+                    } else *(float4_t *)(a.part + left * D + at4 * 4) = o;
                 }
             }
         }
         __syncthreads();
-        x += (uint64_t)(to - from);
+        x += (uint32_t)(to - from);
     }
 }
 
-// Results of pairs that several workgroups share, put together: a workgroup a row, query head and 64 values. Its sixteen groups of threads
-// take the partial results in turn.
+// Results of pairs that several workgroups share, put together by as many: of the pair's results, workgroup w takes its part, and its threads share
+// what the others left of them. A pair of 256 shares (8 rows of 256 values, 131072 tokens) costs a thread two loads, as one of two shares does.
 template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args &a) {
-    __shared__ Plan plan;
-    __shared__ float so[16][64], sm[16], sl[16];
-    const qwk_kv &c = a.c;
-    const int group = (int)a.group, window = (int)a.window, D = (int)c.dim;
-    const uint64_t T = make_plan<QT>(plan, c, group, window), g = shares_of(T, a.grid);
-    const uint32_t row = blockIdx.x, qh = blockIdx.z;
-    uint32_t i;
-    Slot s;
-    if (!slot_find(c, row, i, s)) return;
-    const uint32_t head = qh / a.group;
-    const int mr = ((int)row - s.first) * group + (int)(qh % a.group), blk = mr / (16 * QT);
-    const uint64_t base = i ? plan.end[i - 1] : 0, per_head = (plan.end[i] - base) / c.heads;
-    uint64_t x = base + head * per_head;
-    Range r = block_range<QT>(s, 0, group, window);
-    for (int b = 0; b < blk; b++) x += (uint64_t)r.cnt, r = block_range<QT>(s, b + 1, group, window);
-    const uint32_t w0 = owner_of(x, T, g), w1 = owner_of(x + (uint64_t)r.cnt - 1, T, g);
-    if (w0 == w1) return; // written already
-    const int sub = threadIdx.x / 16, v0 = (int)blockIdx.y * 64 + (int)(threadIdx.x % 16) * 4;
+    __shared__ float4_t so[QW_WG_JOIN];
+    __shared__ float sm[QW_WG_JOIN], sl[QW_WG_JOIN];
+    const uint32_t D4 = a.c.dim / 4, t = threadIdx.x;
     const float neg = -__builtin_inff();
-    float top = neg, sum = 0;
-    float4_t o = {0, 0, 0, 0};
-    for (uint32_t w = w0 + (uint32_t)sub; w <= w1; w += 16) {
-        const size_t at = ((size_t)w * 2 + (w == w0)) * 16 * QT + (mr - blk * 16 * QT);
-        const float mw = a.ml[at * 2], lw = a.ml[at * 2 + 1];
-        const float4_t ow = *(const float4_t *)(a.part + at * D + v0);
-        if (mw == neg) continue;
+    const Part p = ((const Part *)a.parts)[blockIdx.x * 2 + blockIdx.y];
+    if (!p.rows) return;
+    const uint32_t np = p.w1 - p.w0 + 1, all = p.rows * D4, k = blockIdx.x - p.w0;
+    const uint32_t o1 = (k + 1) * all / np;
+    // one with what another left
+    const auto add = [&](float &top, float &sum, float4_t &o, float mw, float lw, float4_t ow) {
+        if (mw == neg) return;
         const float now = fmaxf(top, mw), f = top == neg ? 0.f : __builtin_amdgcn_exp2f(top - now), fw = __builtin_amdgcn_exp2f(mw - now);
         top = now, sum = sum * f + lw * fw, o = o * f + ow * fw;
+    };
+    for (uint32_t o0 = k * all / np; o0 < o1; o0 += QW_WG_JOIN) { // quads of results [o0, o1), at most as many as there are threads
+        const uint32_t n = min(o1 - o0, QW_WG_JOIN), sub = t / n, mine = o0 + t - sub * n; // each by `lanes` threads
+        uint32_t lanes = QW_WG_JOIN / n;
+        const uint32_t row = mine / D4, at4 = mine - row * D4;
+        float top = neg, sum = 0;
+        float4_t o = {0, 0, 0, 0};
+        if (sub < lanes)
+            for (uint32_t w = p.w0 + sub; w <= p.w1; w += lanes) {
+                const size_t at = ((size_t)w * 2 + (w == p.w0)) * 16 * QT + row;
+                add(top, sum, o, a.ml[at * 2], a.ml[at * 2 + 1], *(const float4_t *)(a.part + at * a.c.dim + at4 * 4));
+            }
+        while (lanes > 1) {
+            const uint32_t half = (lanes + 1) / 2;
+            __syncthreads();
+            if (sub >= half && sub < lanes) so[t] = o, sm[t] = top, sl[t] = sum;
+            __syncthreads();
+            if (sub + half < lanes) add(top, sum, o, sm[t + half * n], sl[t + half * n], so[t + half * n]);
+            lanes = half;
+        }
+        if (t < n) {
+            const int mr = (int)(p.m0 + row), j = by(a.by_group, mr);
+            half4_t h;
+            for (int v = 0; v < 4; v++) h[v] = (_Float16)(top == neg ? 0.f : o[v] / sum);
+            *(half4_t *)(a.out + (size_t)(p.row0 + (uint32_t)j) * a.out_stride + ((size_t)p.head * a.group + (uint32_t)(mr - j * (int)a.group)) * a.c.dim + at4 * 4) = h;
+        }
     }
-    *(float4_t *)&so[sub][(threadIdx.x % 16) * 4] = o;
-    if (threadIdx.x % 16 == 0) sm[sub] = top, sl[sub] = sum;
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    top = neg, sum = 0;
-    for (int k = 0; k < 16; k++) top = fmaxf(top, sm[k]);
-    float v = 0;
-    for (int k = 0; k < 16; k++) {
-        if (sm[k] == neg) continue;
-        const float f = __builtin_amdgcn_exp2f(sm[k] - top);
-        sum += sl[k] * f, v += so[k][threadIdx.x] * f;
-    }
-    a.out[(size_t)row * a.out_stride + (size_t)qh * D + blockIdx.y * 64 + threadIdx.x] = __builtin_bit_cast(uint16_t, (_Float16)(top == neg ? 0.f : v / sum));
 }
 
 #define QW_ATTN(TYPE, D, QT, PER) \
@@ -447,7 +548,7 @@ QW_JOIN(2)
 // The unit that holds token `token` of slot i; null: it has no page.
 __device__ __forceinline__ uint8_t *unit_of(const qwk_kv &c, uint32_t i, int token, uint32_t head) {
     const uint64_t at = (uint64_t)i * c.max_pages + ((uint32_t)token >> c.page_log2);
-    const uint32_t page = token < 0 ? 0xffffffffu : c.table[at], pu = c.page_log2 - 4;
+    const uint32_t page = token < 0 ? 0xffffffffu : words(c.table)[at], pu = c.page_log2 - 4;
     return page < c.pages ? c.cache + page * c.page_bytes + (((size_t)head << pu) + ((uint32_t)token >> 4 & ((1u << pu) - 1))) * c.unit : nullptr;
 }
 // Where value v of token t (of its unit) lies: bytes into the unit.

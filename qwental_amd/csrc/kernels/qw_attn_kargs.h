@@ -16,11 +16,16 @@ typedef struct { /* a layer's cache and a step's rows, as every kernel of them t
     uint32_t slots, rows, max_pages, pages, page_log2, heads, dim, unit; /* unit: bytes */
 } qwk_kv;
 
+typedef struct { uint32_t mul, shift; } qwk_div; /* x / d = (x * mul >> 32) >> shift for x < 2^31; mul 0: d is 1 */
+
+#define QW_ATTN_PART 32u /* bytes of what a workgroup says of its share of a pair */
 typedef struct {
     qwk_kv c;
     const uint16_t *q;
     uint16_t *out;
     float *part, *ml; /* partial results: [2 grid][16 QT][dim], and of each row its maximum and its sum */
+    void *parts;      /* [2 grid] */
+    qwk_div by_group;
     uint32_t q_stride, out_stride, group, window, grid;
     float scale; /* of a score, log2(e) in it */
 } qwk_attn_args;

@@ -4,8 +4,6 @@
 // logit, and of the tokens that have exactly that one the first few. It is found by selecting digits of the logits' bits, eight at a time, from
 // histograms of counts (top-k) or weights (top-p); nothing is sorted. Weights are whole numbers, 2^43 times exp((l - max) / temperature): their sums do
 // not depend on the order in which they are made, so neither does the token.
-typedef unsigned long long u64;
-
 // Bits that order as the logits do; 0 for NaN, which is never drawn (nor is minus infinity: its weight is 0).
 __device__ __forceinline__ uint32_t key_of(float l) {
     const uint32_t b = __builtin_bit_cast(uint32_t, l + 0.f); // (-0 is 0)
