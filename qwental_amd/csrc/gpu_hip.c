@@ -231,6 +231,7 @@ static const qw_wg_rule wg_rules[] = {
     {"qwk_attn_join", QW_WG_JOIN, 0, 0},
     {"qwk_attn_", QW_WG_ATTN, 0, 0},
     {"qwk_kv_", QW_WG_KV, 0, 0},
+    {"qwk_sample_bins", QW_WG_SAMPLE_BINS, 0, 0},
     {"qwk_sample", QW_WG_SAMPLE, 0, 0},
 };
 static const qw_wg_rule *wg_rule(const char *fname) {
@@ -2570,7 +2571,10 @@ static bool tr_attn(qw_batch *b) {
     return true;
 }
 // Bindings: 0 logits, 1 parameters, 2 u, 3 ids, 4 probs, 5 ws, 10 qw_sample_geo.
-size_t qw_sample_ws_bytes(const qw_gpu *g, int rows, int vocab) { return !g || rows < 1 || rows > QW_KV_MAX_ROWS || vocab < 1 || vocab > (int)QW_SAMPLE_VOCAB ? 0 : 16; }
+enum { QW_SAMPLE_TILE_BYTES = 8 + QW_SAMPLE_BINS * 8 + QW_SAMPLE_STARTS * 2 + QW_SAMPLE_TILE * 2 }; // of the workspace
+size_t qw_sample_ws_bytes(const qw_gpu *g, int rows, int vocab) {
+    return !g || rows < 1 || rows > QW_KV_MAX_ROWS || vocab < 1 || vocab > (int)QW_SAMPLE_VOCAB ? 0 : ((size_t)rows * cdiv((unsigned)vocab, QW_SAMPLE_TILE) * QW_SAMPLE_TILE_BYTES + 255) / 256 * 256;
+}
 static bool tr_sample(qw_batch *b) {
     qw_sample_geo x;
     qwk_sample_args a = {0};
@@ -2582,7 +2586,14 @@ static bool tr_sample(qw_batch *b) {
     if (!bind_ptr(b, 0, ((R - 1) * (size_t)stride + (size_t)x.vocab) * 4, false, "logits", (void **)&a.logits) || !bind_ptr(b, 1, R * sizeof(qwk_sample_row), false, "parameters", (void **)&a.p) ||
         !bind_ptr(b, 2, R * 4, false, "u", (void **)&a.u) || !bind_whole(b, 3, R * 4, "ids", (void **)&a.ids) || (b->buf[4].h && !bind_whole(b, 4, R * 4, "probs", (void **)&a.probs))) return false;
     if ((uintptr_t)a.logits % 4 || (uintptr_t)a.p % 4 || (uintptr_t)a.u % 4 || (uintptr_t)a.ids % 4 || (uintptr_t)a.probs % 4) return fail(b, "sample_rows: every buffer must be 4-byte aligned");
-    a.vocab = (uint32_t)x.vocab, a.stride = (uint32_t)stride;
+    a.vocab = (uint32_t)x.vocab, a.stride = (uint32_t)stride, a.tiles = cdiv(a.vocab, QW_SAMPLE_TILE);
+    void *ws;
+    if (!bind_ptr(b, 5, qw_sample_ws_bytes(b->g, x.rows, x.vocab), true, "workspace", &ws)) return false;
+    if ((uintptr_t)ws % 16) return fail(b, "sample_rows: the workspace must be 16-byte aligned");
+    const size_t n = R * a.tiles; // the tiles' tokens first: the others' sizes keep 16 bytes for none of them
+    a.order = ws, a.start = a.order + n * QW_SAMPLE_TILE, a.weight = (uint64_t *)(a.start + n * QW_SAMPLE_STARTS), a.head = a.weight + n * QW_SAMPLE_BINS;
+    if (!add_launch(b, "qwk_sample_bins", (unsigned)x.rows, QW_WG_SAMPLE_BINS, &a, sizeof a)) return false;
+    b->l[b->nl - 1].gy = a.tiles;
     return add_launch(b, "qwk_sample", (unsigned)x.rows, QW_WG_SAMPLE, &a, sizeof a);
 }
 qw_kernel *qw_hip_attn_kernel(qw_batch *b, int which) {

@@ -52,10 +52,15 @@ typedef struct {
     const float *u;
     uint32_t *ids;
     float *probs; /* may be NULL */
-    uint32_t vocab, stride;
+    uint64_t *head, *weight; /* of each tile of a row: its largest logit (bits that order as it does) and which token has it; the weights of its bins */
+    uint16_t *start, *order; /* of each tile: where its bins begin in order; its tokens, bin after bin */
+    uint32_t vocab, stride, tiles;
 } qwk_sample_args;
 #define QW_WG_SAMPLE 1024u
-#define QW_SAMPLE_TILE 4096u      /* tokens of which a row keeps the sum */
+#define QW_WG_SAMPLE_BINS 512u
+#define QW_SAMPLE_TILE 8192u      /* tokens of a workgroup of the first launch */
+#define QW_SAMPLE_BINS 256u
+#define QW_SAMPLE_STARTS 264u     /* QW_SAMPLE_BINS + 1, and to a multiple of eight */
 #define QW_SAMPLE_VOCAB (1u << 20) /* at most */
 
 /* What the functions of include/qw_attn.h hand a dispatch beside its buffers, as inline bytes at index QW_ATTN_GEO. */

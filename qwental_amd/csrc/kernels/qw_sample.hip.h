@@ -12,12 +12,18 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 __device__ __forceinline__ float of_key(uint32_t k) { return __builtin_bit_cast(float, k >> 31 ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t KEY_LOWEST = 0x007fffffu; // minus infinity
 
-struct Weigh { // of a row: weights of its tokens
-    double top, c; // largest logit, log2(e) / temperature
-    bool inf;      // the largest is infinity: such tokens share all of it
+// Weights of a row's tokens as whole numbers, 2^43 times 2^(log2(e) l / temperature - octave), where `octave` is the next whole number above what the largest logit gives: those of
+// a tile of the row, relative to its own largest, become the row's by a shift.
+struct Weigh {
+    double top, c, part, octave; // largest logit, log2(e) / temperature, and top c = octave + part, -1 < part <= 0
+    bool inf;                    // the largest is infinity: such tokens share all of it
+    __device__ __forceinline__ Weigh(float largest, float temperature) : top((double)largest), c(1.4426950408889634 / (double)temperature), inf(largest == __builtin_inff()) {
+        // (Where top c is so large that its fraction is lost, two different logits lie 64 octaves apart.)
+        octave = ceil(top * c), part = fabs(octave) < 0x1p30 ? top * c - octave : 0;
+    }
     __device__ __forceinline__ u64 operator()(float l) const {
         if (inf) return l == __builtin_inff() ? 1ull << 43 : 0;
-        const double x = ((double)l - top) * c; // in 64 bits: a 24-bit product would cost a small weight its last digits
+        const double x = ((double)l - top) * c + part; // in 64 bits: a 24-bit product would cost a small weight its last digits
         if (!(x > -64.)) return 0;
         const float i = __builtin_rintf((float)x), f = __builtin_amdgcn_exp2f((float)(x - (double)i));
         return (u64)__builtin_ldexpf(f, (int)i + 43);
@@ -95,7 +101,7 @@ __device__ __forceinline__ void sample_row(SampleShared &s, const qwk_sample_arg
         if (t == 0 && a.probs) a.probs[row] = top <= KEY_LOWEST ? 0.f : 1.f;
         return;
     }
-    const Weigh weigh = {(double)of_key(top), 1.4426950408889634 / (double)p.temperature, of_key(top) == __builtin_inff()};
+    const Weigh weigh(of_key(top), p.temperature);
     uint32_t border = KEY_LOWEST + 1, equal = 0, keep = 0; // tokens above `border`, and the first `keep` of the `equal` ones that lie on it (equal 0: all of them)
     if (p.top_k && p.top_k < a.vocab) {
         uint32_t prefix = 0;
@@ -132,7 +138,7 @@ __device__ __forceinline__ void sample_row(SampleShared &s, const qwk_sample_arg
         }
         last = ~prefix & 0xffffff;
     }
-    const u64 least = p.min_p > 0 ? (u64)((double)fminf(p.min_p, 1.f) * 0x1p43) : 0;
+    const u64 least = p.min_p > 0 ? (u64)((double)fminf(p.min_p, 1.f) * (double)weigh(of_key(top))) : 0;
     const auto weight = [&](uint32_t i) -> u64 {
         if (i >= a.vocab) return 0;
         const float x = l[i];
@@ -177,7 +183,426 @@ __device__ __forceinline__ void sample_row(SampleShared &s, const qwk_sample_arg
                 if (a.probs) a.probs[row] = (float)((double)w[k] / (double)all);
             }
 }
+
+// The fast way: two launches. qwk_sample_bins, a workgroup for 8192 logits, deals them into bins of 1/8 from its own largest logit down (the bins' borders are
+// the same for all tiles: floor(8 l)), and leaves each bin's weight (relative to the tile's largest) and its tokens. qwk_sample, a workgroup a row, adds
+// the tiles' bins up; then a filter's border lies in a bin whose tokens are known, some thousand of them at most as a rule: 256 finer bins, then each of the few in one of these
+// against all others. The token drawn is found by the tiles' sums and one tile. A border in the last bin (what lies 31 below the largest), or in a bin or finer bin of too many
+// tokens, goes the slow way (sample_row).
+constexpr uint32_t REST = QW_SAMPLE_BINS - 1, LIST = 8192, FEW = 1024, NEAR = 1024, NEAR_TILES = 32, TILES = QW_SAMPLE_VOCAB / QW_SAMPLE_TILE;
+__device__ __forceinline__ int grid_of(float l) { return (int)fminf(fmaxf(floorf(l * 8.f), -1e9f), 1e9f); }
+__device__ __forceinline__ uint32_t finer(float l, int g) { return 255u - (uint32_t)fminf(fmaxf((l * 8.f - (float)g) * 256.f, 0.f), 255.f); } // within a bin, from its top down
+
+// Sums over the lanes up to and with this one.
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 lanes_below(u64 x) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, false);
+    return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 wave_up(u64 x) {
+    x += lanes_below<0x111, 0xf>(x); // row_shr:1, 2, 4, 8
+    x += lanes_below<0x112, 0xf>(x);
+    x += lanes_below<0x114, 0xf>(x);
+    x += lanes_below<0x118, 0xf>(x);
+    x += lanes_below<0x142, 0xa>(x); // row_bcast:15, 31
+    x += lanes_below<0x143, 0xc>(x);
+    return x;
+}
+__device__ __forceinline__ u64 of_lane(u64 x, int lane) { return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane); }
+
+extern "C" __global__ __launch_bounds__(QW_WG_SAMPLE_BINS) void qwk_sample_bins(qwk_sample_args a) {
+    constexpr uint32_t N = QW_SAMPLE_TILE / QW_WG_SAMPLE_BINS;
+    __shared__ u64 weight[QW_SAMPLE_BINS];
+    __shared__ uint32_t count[QW_SAMPLE_BINS], from[QW_SAMPLE_BINS];
+    __shared__ u64 part[QW_WG_SAMPLE_BINS / 64];
+    __shared__ alignas(16) uint16_t order[QW_SAMPLE_TILE];
+    const uint32_t t = threadIdx.x, tile = blockIdx.y, row = blockIdx.x, base = tile * QW_SAMPLE_TILE;
+    const float *l = a.logits + (size_t)row * a.stride;
+    const qwk_sample_row p = a.p[row];
+    float x[N];
+    u64 best = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) {
+        const uint32_t i = base + k * QW_WG_SAMPLE_BINS + t;
+        x[k] = i < a.vocab ? l[i] : -__builtin_inff();
+    }
+    for (uint32_t i = t; i < QW_SAMPLE_BINS; i += QW_WG_SAMPLE_BINS) weight[i] = 0, count[i] = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) {
+        const uint32_t i = base + k * QW_WG_SAMPLE_BINS + t;
+        const u64 o = (u64)key_of(x[k]) << 32 | ~i;
+        best = i < a.vocab && o > best ? o : best;
+    }
+    for (int d = 32; d; d >>= 1) {
+        const u64 o = __shfl_xor(best, d);
+        best = o > best ? o : best;
+    }
+    if (t % 64 == 0) part[t / 64] = best;
+    __syncthreads();
+    for (uint32_t i = 0; i < QW_WG_SAMPLE_BINS / 64; i++) best = part[i] > best ? part[i] : best;
+    const size_t at = (size_t)row * a.tiles + tile;
+    if (t == 0) a.head[at] = best;
+    const float top = of_key((uint32_t)(best >> 32));
+    if ((uint32_t)(best >> 32) <= KEY_LOWEST || top == __builtin_inff() || !(p.temperature > 0) || p.top_k == 1) return; // (the second launch does not ask for more)
+    const Weigh weigh(top, p.temperature);
+    const int g = grid_of(top);
+    uint32_t bin[N], rank[N];
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) {
+        const uint32_t i = base + k * QW_WG_SAMPLE_BINS + t;
+        bin[k] = x[k] == x[k] ? (uint32_t)min((int64_t)g - grid_of(x[k]), (int64_t)REST) : REST;
+        if (i >= a.vocab) continue;
+        rank[k] = atomicAdd(&count[bin[k]], 1u);
+        const u64 w = weigh(x[k]);
+        if (w) atomicAdd(&weight[bin[k]], w);
+    }
+    __syncthreads();
+    if (t < 64) { // some bins a lane
+        constexpr uint32_t K = QW_SAMPLE_BINS / 64;
+        uint32_t n[K], sum = 0;
+        for (uint32_t k = 0; k < K; k++) n[k] = sum, sum += count[t * K + k];
+        const uint32_t before = (uint32_t)wave_up(sum) - sum;
+        for (uint32_t k = 0; k < K; k++) from[t * K + k] = before + n[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) {
+        const uint32_t i = k * QW_WG_SAMPLE_BINS + t;
+        if (base + i < a.vocab) order[from[bin[k]] + rank[k]] = (uint16_t)i;
+    }
+    __syncthreads();
+    uint16_t *start = a.start + at * QW_SAMPLE_STARTS;
+    for (uint32_t i = t; i < QW_SAMPLE_BINS; i += QW_WG_SAMPLE_BINS) start[i] = (uint16_t)from[i], a.weight[at * QW_SAMPLE_BINS + i] = weight[i];
+    if (t == 0) start[QW_SAMPLE_BINS] = (uint16_t)min(a.vocab - base, QW_SAMPLE_TILE);
+    const uint4 *from4 = (const uint4 *)order;
+    for (uint32_t i = t; i < QW_SAMPLE_TILE / 8; i += QW_WG_SAMPLE_BINS) ((uint4 *)(a.order + at * QW_SAMPLE_TILE))[i] = from4[i];
+}
+
+struct SampleFast {
+    u64 weight[QW_SAMPLE_BINS], fine_weight[FEW], few_weight[FEW], sum[TILES], part[16], pick_at, all, below;
+    uint32_t count[QW_SAMPLE_BINS], fine_count[FEW], key[LIST], id[LIST], few_key[FEW], few_id[FEW], pos[TILES], from[TILES], many[TILES], shift[TILES];
+    int off[TILES]; // bins that a tile's first lies below the row's; shift: of its weights, by octaves
+    uint16_t starts[NEAR_TILES * (QW_SAMPLE_BINS + 1)]; // of up to so many tiles, and the tokens of their first bins
+    uint32_t near_key[NEAR], near_id[NEAR];
+    uint32_t n, few, pick, cut_key, cut_id, slow, which;
+    u64 before_n, before_w;
+};
+
+struct FastSampler {
+    SampleFast &s;
+    const qwk_sample_args &a;
+    const float *l;
+    const Weigh weigh;
+    const size_t first_tile;
+    const int g;         // grid_of the largest logit
+    const uint32_t near; // tokens of each tile that are at hand
+    int loaded = -1;
+
+    // Of N bins from the first on, the one in which the sum reaches `want` (the last one that holds anything, if none does): pick, and what lies before it.
+    template <int N> __device__ void find(const u64 *weight, const uint32_t *count, bool weights, u64 want) {
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            constexpr int K = N / 64;
+            u64 w = 0, n = 0;
+            int last = -1;
+            for (int k = 0; k < K; k++) {
+                w += weight[threadIdx.x * K + k], n += count[threadIdx.x * K + k];
+                if (count[threadIdx.x * K + k]) last = (int)threadIdx.x * K + k;
+            }
+            const u64 uw = wave_up(w), un = wave_up(n);
+            const u64 hit = __ballot((weights ? uw : un) >= want && n), any = __ballot(last >= 0);
+            const uint32_t lane = hit ? (uint32_t)__builtin_ctzll(hit) : any ? 63u - (uint32_t)__builtin_clzll(any) : 0;
+            if (threadIdx.x == lane) {
+                u64 bw = uw - w, bn = un - n;
+                int k = 0;
+                while ((int)lane * K + k < last) {
+                    const u64 ww = weight[lane * K + k], nn = count[lane * K + k];
+                    if ((weights ? bw + ww : bn + nn) >= want && nn) break;
+                    bw += ww, bn += nn, k++;
+                }
+                s.pick = lane * K + (uint32_t)k, s.before_w = bw, s.before_n = bn;
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ uint32_t starts(uint32_t tile, int bin) const { return near ? s.starts[tile * (QW_SAMPLE_BINS + 1) + (uint32_t)bin] : a.start[(first_tile + tile) * QW_SAMPLE_STARTS + (uint32_t)bin]; }
+    // The tokens of a bin of the row's, into the list; false: more than it holds.
+    __device__ bool load(int bin) {
+        if (bin == loaded) return true;
+        const uint32_t t = threadIdx.x;
+        __syncthreads();
+        if (t < 64) {
+            uint32_t base = 0;
+            for (uint32_t from = 0; from < a.tiles; from += 64) {
+                const uint32_t tile = from + t;
+                const int b = tile < a.tiles ? bin - s.off[tile] : -1;
+                uint32_t n0 = 0, n1 = 0;
+                if (b >= 0) n0 = starts(tile, b), n1 = starts(tile, b + 1);
+                const uint32_t up = base + (uint32_t)wave_up(n1 - n0);
+                if (tile < a.tiles) s.from[tile] = n0, s.many[tile] = n1 - n0, s.pos[tile] = up - (n1 - n0);
+                base = (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
+            }
+            if (t == 0) s.n = base;
+        }
+        __syncthreads();
+        if (s.n > LIST) return false;
+        for (uint32_t tile = t / 32; tile < a.tiles; tile += QW_WG_SAMPLE / 32)
+            for (uint32_t i = t % 32; i < s.many[tile]; i += 32) {
+                const uint32_t at = s.from[tile] + i;
+                uint32_t id, key;
+                if (at < near) id = s.near_id[tile * near + at], key = s.near_key[tile * near + at];
+                else id = tile * QW_SAMPLE_TILE + a.order[(first_tile + tile) * QW_SAMPLE_TILE + at], key = key_of(l[id]);
+                s.id[s.pos[tile] + i] = id, s.key[s.pos[tile] + i] = key;
+            }
+        __syncthreads();
+        loaded = bin;
+        return true;
+    }
+    // The border of a filter: the last token kept, of those that `want` tokens (or weight) reach. Leaves it in cut_key and cut_id, and what it and those before it weigh in all.
+    __device__ bool border(bool weights, u64 want) {
+        const uint32_t t = threadIdx.x;
+        find<QW_SAMPLE_BINS>(s.weight, s.count, weights, want);
+        const int bin = (int)s.pick;
+        const u64 bn = s.before_n, bw = s.before_w;
+        if (bin == (int)REST || !load(bin)) return false;
+        u64 fn = bn, fw = bw;
+        if (t == 0) s.few = 0, s.pick_at = 0;
+        if (s.n <= 64) { // few enough as they are
+            if (t < s.n) s.few_key[t] = s.key[t], s.few_id[t] = s.id[t], s.few_weight[t] = weigh(of_key(s.key[t]));
+            __syncthreads();
+            if (t == 0) s.few = s.n;
+        } else {
+            if (t < 256) s.fine_weight[t] = 0, s.fine_count[t] = 0;
+            __syncthreads();
+            for (uint32_t i = t; i < s.n; i += QW_WG_SAMPLE) {
+                const float x = of_key(s.key[i]);
+                const uint32_t f = finer(x, g - bin);
+                atomicAdd(&s.fine_count[f], 1u);
+                const u64 w = weigh(x);
+                if (w) atomicAdd(&s.fine_weight[f], w);
+            }
+            find<256>(s.fine_weight, s.fine_count, weights, want - (weights ? bw : bn));
+            const uint32_t f = s.pick;
+            fn += s.before_n, fw += s.before_w;
+            for (uint32_t i = t; i < s.n; i += QW_WG_SAMPLE) {
+                const float x = of_key(s.key[i]);
+                if (finer(x, g - bin) != f) continue;
+                const uint32_t k = atomicAdd(&s.few, 1u);
+                if (k < FEW) s.few_key[k] = s.key[i], s.few_id[k] = s.id[i], s.few_weight[k] = weigh(x);
+            }
+        }
+        __syncthreads();
+        if (s.few > FEW) return false;
+        // each against all others, by as many threads as there are for it
+        const uint32_t few = s.few, each = few <= 64 ? 64 : few <= 256 ? 256 : FEW, j = t % each, parts = QW_WG_SAMPLE / each;
+        const uint32_t key = j < few ? s.few_key[j] : 0, id = j < few ? s.few_id[j] : 0;
+        if (t < each) s.fine_weight[t] = 0, s.fine_count[t] = 0;
+        u64 n = 0, w = 0;
+#pragma unroll 4
+        for (uint32_t i = t / each; i < few; i += parts) {
+            const uint32_t k = s.few_key[i], d = s.few_id[i];
+            const u64 x = s.few_weight[i];
+            const bool before = k > key || (k == key && d < id);
+            n += before, w += before ? x : 0;
+        }
+        __syncthreads();
+        if (n) atomicAdd(&s.fine_count[j], (uint32_t)n), atomicAdd(&s.fine_weight[j], w);
+        __syncthreads();
+        n = fn + s.fine_count[j], w = fw + s.fine_weight[j];
+        if (t < few && (weights ? w : n) < want) atomicMax(&s.pick_at, (n - fn + 1) << 32 | t); // the last of those that begin before it
+        __syncthreads();
+        if (!s.pick_at) return false;
+        if (t == (uint32_t)s.pick_at) s.cut_key = s.few_key[t], s.cut_id = s.few_id[t], s.all = w + s.few_weight[t];
+        __syncthreads();
+        return true;
+    }
+};
+
+// false: the slow way has to be taken
+__device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t row) {
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const qwk_sample_row p = a.p[row];
+    const float *l = a.logits + (size_t)row * a.stride;
+    const size_t first_tile = (size_t)row * a.tiles;
+    const u64 mine = t < a.tiles ? a.head[first_tile + t] : 0;
+    u64 best = mine;
+    for (int d = 32; d; d >>= 1) {
+        const u64 o = __shfl_xor(best, d);
+        best = o > best ? o : best;
+    }
+    if (lane == 0) s.part[wave] = best;
+    for (uint32_t i = t; i < QW_SAMPLE_BINS; i += QW_WG_SAMPLE) s.weight[i] = 0, s.count[i] = 0;
+    __syncthreads();
+    for (uint32_t i = 0; i < QW_WG_SAMPLE / 64; i++) best = s.part[i] > best ? s.part[i] : best;
+    const uint32_t top_key = (uint32_t)(best >> 32);
+    const float top = of_key(top_key);
+    if (top_key <= KEY_LOWEST || !(p.temperature > 0) || p.top_k == 1) { // nothing to draw from, or no chance in it
+        if (t == 0) a.ids[row] = top_key <= KEY_LOWEST ? 0xffffffffu : ~(uint32_t)best;
+        if (t == 0 && a.probs) a.probs[row] = top_key <= KEY_LOWEST ? 0.f : 1.f;
+        return true;
+    }
+    if (top == __builtin_inff()) return false;
+    const Weigh weigh(top, p.temperature);
+    const int g = grid_of(top);
+    if (t < a.tiles) {
+        const uint32_t k = (uint32_t)(mine >> 32);
+        const float m = of_key(k);
+        const bool none = k <= KEY_LOWEST; // (such a tile has left no bins)
+        s.off[t] = none ? 1 << 30 : (int)min((int64_t)g - grid_of(m), (int64_t)1 << 30);
+        s.shift[t] = none ? 63 : (uint32_t)fmin(weigh.octave - ceil((double)m * weigh.c), 63.);
+    }
+    __syncthreads();
+    // A thread a bin of every fourth tile; four tiles' loads at once, wanted or not (one after the other behind a look at the bin's count: 20 us of 31).
+    constexpr uint32_t EVERY = QW_WG_SAMPLE / QW_SAMPLE_BINS;
+    // Beside them the first tokens of every tile's order, a thread each: a border among the row's first some hundred tokens then costs no round trips of its own.
+    const uint32_t near = a.tiles <= NEAR / 64 ? 64 : a.tiles <= NEAR_TILES ? NEAR / NEAR_TILES : 0;
+    uint32_t near_id = 0, near_key = 0;
+    if (near && t < near * a.tiles) {
+        const uint32_t tile = t / near, i = t % near, in = min(a.vocab - tile * QW_SAMPLE_TILE, QW_SAMPLE_TILE);
+        const uint32_t at = i < in ? a.order[(first_tile + tile) * QW_SAMPLE_TILE + i] : 0;
+        near_id = tile * QW_SAMPLE_TILE + min(at, in - 1); // (a tile without bins has left no order)
+        near_key = key_of(l[near_id]);
+    }
+    const uint32_t bin = t % QW_SAMPLE_BINS;
+    for (uint32_t from = t / QW_SAMPLE_BINS; from < a.tiles; from += 4 * EVERY) {
+        uint32_t n0[4], n1[4];
+        u64 w[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const size_t tile = first_tile + min(from + k * EVERY, a.tiles - 1);
+            n0[k] = a.start[tile * QW_SAMPLE_STARTS + bin], n1[k] = a.start[tile * QW_SAMPLE_STARTS + bin + 1], w[k] = a.weight[tile * QW_SAMPLE_BINS + bin];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint32_t tile = from + k * EVERY;
+            if (tile >= a.tiles) break;
+            if (near) {
+                s.starts[tile * (QW_SAMPLE_BINS + 1) + bin] = (uint16_t)n0[k];
+                if (bin == REST) s.starts[tile * (QW_SAMPLE_BINS + 1) + QW_SAMPLE_BINS] = (uint16_t)n1[k];
+            }
+            if (s.off[tile] == 1 << 30) {
+                if (bin == 0) atomicAdd(&s.count[REST], min(a.vocab - tile * QW_SAMPLE_TILE, QW_SAMPLE_TILE));
+                continue;
+            }
+            if (n1[k] == n0[k]) continue;
+            const uint32_t b = min((uint32_t)s.off[tile] + bin, REST);
+            atomicAdd(&s.count[b], n1[k] - n0[k]);
+            const u64 v = w[k] >> s.shift[tile];
+            if (v) atomicAdd(&s.weight[b], v);
+        }
+    }
+    if (near) s.near_id[t] = near_id, s.near_key[t] = near_key;
+    __syncthreads();
+    FastSampler f{s, a, l, weigh, first_tile, g, near};
+    uint32_t cut_key = 0, cut_id = ~0u; // the last token kept
+    int edge = QW_SAMPLE_BINS;          // its bin
+    u64 all = 0;
+    const bool by_count = p.top_k && p.top_k < a.vocab, by_weight = p.top_p < 1;
+    u64 want = p.top_k;
+    if (!by_count && by_weight) {
+        for (uint32_t i = lane; i < QW_SAMPLE_BINS; i += 64) all += s.weight[i];
+        all = of_lane(wave_up(all), 63);
+    }
+#pragma unroll 1
+    for (int pass = by_count ? 0 : 1; pass < (by_weight ? 2 : 1); pass++) { // (one after the other through the same code)
+        if (pass) want = (u64)ceil((double)fmaxf(p.top_p, 1e-30f) * (double)all), want = want < 1 ? 1 : want > all ? all : want;
+        __syncthreads();
+        if (!f.border(pass, want)) return false;
+        all = s.all;
+        if (s.cut_key > cut_key || (s.cut_key == cut_key && s.cut_id < cut_id)) cut_key = s.cut_key, cut_id = s.cut_id, edge = g - grid_of(of_key(cut_key));
+    }
+    u64 least = 0;
+    if (p.min_p > 0) {
+        const float m = fminf(p.min_p, 1.f);
+        least = (u64)((double)m * (double)weigh(top));
+        const double x = weigh.top + (log2((double)m) - 0x1p-23) / weigh.c; // the logit of that weight, less what a weight may be rounded by: at a bin's border the tokens below are looked at too
+        edge = (int)fmin((double)edge, (double)g - floor(x * 8.));
+        if (edge >= (int)REST) return false;
+        edge = edge < 0 ? 0 : edge;
+    }
+    const auto weight = [&](uint32_t key, uint32_t id) -> u64 {
+        if (key < cut_key || (key == cut_key && id > cut_id)) return 0;
+        const u64 w = weigh(of_key(key));
+        return w < least ? 0 : w;
+    };
+    // the tiles' sums: whole bins above the edge's, and those of its tokens that are kept
+    if (edge < (int)QW_SAMPLE_BINS && !f.load(edge)) return false;
+    for (uint32_t tile = t / 32; tile < a.tiles; tile += QW_WG_SAMPLE / 32) {
+        u64 w = 0;
+        const int end = edge < (int)QW_SAMPLE_BINS ? edge - s.off[tile] : (int)QW_SAMPLE_BINS;
+#pragma unroll
+        for (uint32_t k = 0; k < QW_SAMPLE_BINS / 32; k++) {
+            const uint32_t b = k * 32 + t % 32;
+            const u64 x = k * 32 < (uint32_t)max(end, 0) ? a.weight[(first_tile + tile) * QW_SAMPLE_BINS + b] : 0;
+            w += (int)b < end ? x : 0;
+        }
+        for (int d = 16; d; d >>= 1) w += __shfl_xor(w, d);
+        if (t % 32 == 0) s.sum[tile] = s.off[tile] == 1 << 30 ? 0 : w >> s.shift[tile];
+    }
+    __syncthreads();
+    if (edge < (int)QW_SAMPLE_BINS)
+        for (uint32_t i = t; i < s.n; i += QW_WG_SAMPLE) {
+            const u64 w = weight(s.key[i], s.id[i]);
+            if (w) atomicAdd(&s.sum[s.id[i] / QW_SAMPLE_TILE], w);
+        }
+    __syncthreads();
+    if (t < 64) {
+        u64 n[TILES / 64], sum = 0;
+        for (uint32_t k = 0; k < TILES / 64; k++) n[k] = t * (TILES / 64) + k < a.tiles ? s.sum[t * (TILES / 64) + k] : 0, sum += n[k];
+        const u64 up = wave_up(sum), whole = of_lane(up, 63);
+        const double u = (double)a.u[row];
+        const u64 at = u > 0 ? min((u64)(u * (double)whole), whole - 1) : 0;
+        if (t == 0) s.all = whole;
+        u64 below = up - sum;
+        if (below <= at && at < up)
+            for (uint32_t k = 0; k < TILES / 64; below += n[k++])
+                if (below <= at && at < below + n[k]) s.which = t * (TILES / 64) + k, s.below = at - below;
+    }
+    __syncthreads();
+    // in the tile that the draw falls into: 64 tokens a wave at a time, then one of them
+    constexpr uint32_t K = QW_SAMPLE_TILE / QW_WG_SAMPLE, WAVES = QW_WG_SAMPLE / 64;
+    const uint32_t base = s.which * QW_SAMPLE_TILE;
+    u64 w[K], up[K];
+    float x[K];
+#pragma unroll
+    for (uint32_t k = 0; k < K; k++) x[k] = l[min(base + k * QW_WG_SAMPLE + t, a.vocab - 1)];
+#pragma unroll
+    for (uint32_t k = 0; k < K; k++) {
+        const uint32_t id = base + k * QW_WG_SAMPLE + t;
+        w[k] = id < a.vocab ? weight(key_of(x[k]), id) : 0, up[k] = wave_up(w[k]);
+        if (lane == 63) s.fine_weight[k * WAVES + wave] = up[k];
+    }
+    __syncthreads();
+    static_assert(K * WAVES == 128, "two a lane");
+    u64 whole = 0, mine_below[K] = {};
+    {
+        const u64 n0 = s.fine_weight[lane * 2], n1 = s.fine_weight[lane * 2 + 1], u = wave_up(n0 + n1);
+        whole = of_lane(u, 63);
+#pragma unroll
+        for (uint32_t k = 0; k < K; k++) { // what lies before this wave's k-th group
+            const uint32_t at = k * WAVES + wave;
+            mine_below[k] = of_lane(u, (int)(at / 2)) - of_lane(at % 2 ? n1 : n0 + n1, (int)(at / 2));
+        }
+    }
+    if (!whole) return false;
+    const u64 at = min((u64)s.below, whole - 1); // (the tile's bins and its tokens may add up to some units' difference)
+#pragma unroll
+    for (uint32_t k = 0; k < K; k++) {
+        const u64 c = mine_below[k] + up[k];
+        if (c - w[k] <= at && at < c) {
+            a.ids[row] = base + k * QW_WG_SAMPLE + t;
+            if (a.probs) a.probs[row] = (float)((double)w[k] / (double)s.all);
+        }
+    }
+    return true;
+}
+
 extern "C" __global__ __launch_bounds__(QW_WG_SAMPLE) void qwk_sample(qwk_sample_args a) {
-    __shared__ SampleShared s;
-    sample_row(s, a, blockIdx.x);
+    __shared__ union U {
+        SampleShared slow;
+        SampleFast fast;
+        __device__ U() {}
+    } s;
+    if (sample_fast(s.fast, a, blockIdx.x)) return;
+    __syncthreads();
+    sample_row(s.slow, a, blockIdx.x);
 }
