@@ -2514,9 +2514,11 @@ static bool tr_kv_write(qw_batch *b) {
     if (!apart(b, &qo, "q_out", &k, "k") || !apart(b, &qo, "q_out", &v, "v") || !apart(b, &qo, "q_out", &cache, "the cache") || !apart(b, &q, "q", &cache, "the cache") || !apart(b, &k, "k", &cache, "the cache") ||
         !apart(b, &v, "v", &cache, "the cache")) return false;
     a.q_heads = (uint32_t)x.q_heads, a.rot = (uint32_t)x.rot, a.axes = (uint32_t)x.axes, a.pairs0 = (uint32_t)x.pairs[0], a.pairs1 = (uint32_t)x.pairs[1], a.adjacent = x.adjacent != 0;
-    if (!add_launch(b, x.type == 1 ? "qwk_kv_write_f1" : "qwk_kv_write_f8", (unsigned)x.rows, QW_WG_KV, &a, sizeof a)) return false;
-    b->l[b->nl - 1].gy = cdiv((unsigned)(x.q_heads + 2 * x.heads), QW_WG_KV / 64);
-    return true;
+    // A wave a head while that makes no more than eight waves for each SIMD of the device, then several heads a wave: what a row costs before its first head is then shared
+    const unsigned heads = (unsigned)(x.q_heads + 2 * x.heads), waves = (unsigned)b->g->ncu * 32 / (unsigned)x.rows;
+    a.waves = waves < 1 ? 1 : umin(waves, heads);
+    static const char *const names[2][2] = {{"qwk_kv_write_f1_c1", "qwk_kv_write_f1_c2"}, {"qwk_kv_write_f8_c1", "qwk_kv_write_f8_c2"}};
+    return add_launch(b, names[x.type == 8][x.dim > 128], cdiv((unsigned)x.rows * a.waves, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
 }
 static bool tr_kv_read(qw_batch *b) {
     qw_attn_geo x;
@@ -2525,9 +2527,9 @@ static bool tr_kv_read(qw_batch *b) {
     if (!kv_bind(b, &x, &a.c, false, &cache)) return false;
     if (!kv_rows(b, 6, true, &x, x.heads, x.stride[2], "k", &a.k, &a.k_stride, &k) || !kv_rows(b, 7, true, &x, x.heads, x.stride[3], "v", &a.v, &a.v_stride, &v)) return false;
     if (!apart(b, &k, "k", &v, "v") || !apart(b, &k, "k", &cache, "the cache") || !apart(b, &v, "v", &cache, "the cache")) return false;
-    if (!add_launch(b, x.type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", (unsigned)x.rows, QW_WG_KV, &a, sizeof a)) return false;
-    b->l[b->nl - 1].gy = cdiv((unsigned)x.heads, QW_WG_KV / 64);
-    return true;
+    // a wave a unit and head, for keys and for values: 16 rows a unit, and for every slot one begun and one ended within a unit
+    const unsigned units = (unsigned)x.rows / QW_UNIT + 2 * umin((unsigned)x.slots, (unsigned)x.rows);
+    return add_launch(b, x.type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", cdiv(units * 2 * (unsigned)x.heads, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
 }
 // Two workgroups a compute unit; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
 static unsigned attn_grid(const qw_gpu *g) { return 2 * (unsigned)g->ncu; }

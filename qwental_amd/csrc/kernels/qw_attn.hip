@@ -20,11 +20,12 @@ enum { F16 = 1, Q8 = 8 };
 // for tokens 4 (lane >> 4) + i, which is what the second product takes from that lane. Nothing moves between lanes and nothing goes
 // through LDS between the two; the cache's units are stored so that a lane's operands are 16 consecutive bytes of a wave's 1024.
 //
-// Work: a pair is (slot, head, block of 16 QT of the slot's rows x query heads of that head); its tiles of 32 tokens lie one behind another,
-// pair after pair, and the workgroups of the grid take equal shares of that line, wherever pairs begin or end in it: a long slot is
-// cut over many workgroups, short ones share one. All of it follows from first[] and len[] on the device, so a captured call goes on
-// being right (and even) as the slots grow. A share that ends inside a pair leaves (maximum, sum, unnormalised result), which qwk_attn_join
-// puts together in the order of the shares: the same bits every time.
+// Work: a pair is (slot, head, block of 16 QT of the slot's rows x query heads of that head), with its tiles of 32 tokens. As a rule a pair is cut into as many equal shares as it has
+// times `size` tiles, a workgroup each, with the least `size` (of whole rounds of the four waves) that the grid has workgroups for: nobody then begins twice. Where pairs are many and
+// unlike, that would leave some workgroups with much more than others; their tiles then lie one behind another, pair after pair, and the workgroups take equal shares of that line,
+// wherever pairs begin or end in it (Shares). All of it follows from first[] and len[] on the device, so a captured call goes on being right, and even, as the slots grow. What a
+// share makes of a pair that others have shares of it leaves as (maximum, sum, unnormalised result), and qwk_attn_join puts these together in the order of the shares: the same
+// bits every time.
 
 struct Slot { int n, len, first; }; // rows, tokens, first row
 
@@ -65,8 +66,6 @@ template <int QT> __device__ __forceinline__ Range block_range(const Slot &s, in
 }
 template <int QT> __device__ __forceinline__ int blocks_of(const Slot &s, const qwk_attn_args &a) { return (s.n * (int)a.group + 16 * QT - 1) / (16 * QT); }
 
-// Tiles of all slots, a lane a slot. Every wave makes it and writes it down for itself (all the same, where it is the same LDS): no barrier.
-struct Plan { uint32_t each[QW_KV_SLOTS_MAX], end[QW_KV_SLOTS_MAX]; }; // tiles of one of the slot's heads; of all slots up to and with this one
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) { // sums over the lanes up to and with this one
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false); // row_shr:1, 2, 4, 8
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
@@ -76,10 +75,11 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) { // sums over the lan
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
     return x;
 }
-template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, uint32_t &pairs) { // returns the tiles of all
+// Tiles (size 0) or shares of up to `size` tiles of all slots, a lane a slot. Every wave makes it and writes it down for itself (all the same, where it is the same LDS): no barrier.
+struct Plan { uint32_t each[QW_KV_SLOTS_MAX], end[QW_KV_SLOTS_MAX]; }; // of one of the slot's heads; of all slots up to and with this one
+template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, uint32_t size, uint32_t *pairs) { // returns the whole
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t T = 0;
-    pairs = 0;
+    uint32_t T = 0, P = 0;
 #pragma unroll 1
     for (uint32_t k = 0; k < a.c.slots; k += 64) {
         const uint32_t i = k + lane;
@@ -88,23 +88,21 @@ template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const q
         asm volatile("" : "+v"(s.n), "+v"(s.len)); // (all three loads at once, not the length's behind a branch on the others)
         const int nb = i < a.c.slots ? blocks_of<QT>(s, a) : 0;
 #pragma unroll 1
-        for (int b = 0; b < nb; b++) each += (uint32_t)block_range<QT>(s, b, a).cnt;
+        for (int b = 0; b < nb; b++) {
+            const uint32_t cnt = (uint32_t)block_range<QT>(s, b, a).cnt;
+            each += size ? (cnt + size - 1) / size : cnt;
+        }
         const uint32_t end = T + wave_scan(each * a.c.heads);
         p.each[i] = each, p.end[i] = end;
         T = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
-        pairs += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)nb), 63);
+        if (pairs) P += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)nb), 63);
     }
-    pairs *= a.c.heads;
+    if (pairs) *pairs = P * a.c.heads;
     return T;
 }
-// Shares: workgroup w of g takes the next T / g tiles, the first T % g of them one more.
+// Shares along the line of all tiles: workgroup w of g takes the next T / g tiles, the first T % g of them one more.
 struct Shares {
     uint32_t g, base, more;
-    // As many workgroups as there are four tiles for, one a wave, or pairs: behind its first pair's end a workgroup starts once more (3 us; a slot of one token and four heads: one
-    // workgroup for all of them 15.9 us, four 6)
-    __device__ __forceinline__ Shares(uint32_t T, uint32_t pairs, uint32_t grid) : g(min(grid, max((T + 3) / 4, pairs))), base(0), more(0) {
-        if (g) base = T / g, more = T - base * g;
-    }
     __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * base + min(w, more); }
     __device__ __forceinline__ uint32_t owner(uint32_t x) const {
         const uint32_t big = more * (base + 1);
@@ -337,23 +335,48 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
     const int group = (int)a.group, window = (int)a.window;
     Part *parts = (Part *)a.parts + blockIdx.x * 2;
     __shared__ Plan plan;
-    uint32_t pairs;
-    const uint32_t T = make_plan<QT>(plan, a, pairs);
-    const Shares sh(T, pairs, a.grid);
+    // The least size of a share that the grid is enough for: 4 tiles, or a round more than equal shares of everything would have, or two. (To begin once more in another pair costs a
+    // workgroup some 5 us, as much as two rounds.) Otherwise (size 0) shares of the whole line.
+    uint32_t pairs, size = 0;
+    const uint32_t T = make_plan<QT>(plan, a, 0, &pairs);
+    Shares sh = {0, 0, 0};
+    if (pairs <= a.grid) {
+        const uint32_t least = max(4u, (T + a.grid - 1) / a.grid + 3 & ~3u);
+#pragma unroll 1
+        for (uint32_t k = 0; k < 3 && !size; k++) {
+            sh.g = make_plan<QT>(plan, a, least + 4 * k, nullptr);
+            if (sh.g <= a.grid) size = least + 4 * k;
+        }
+    }
+    if (!size) {
+        if (pairs <= a.grid) make_plan<QT>(plan, a, 0, nullptr);
+        sh.g = min(a.grid, T), sh.base = T / max(sh.g, 1u), sh.more = T - sh.base * sh.g;
+    }
     if (threadIdx.x < 2) parts[threadIdx.x].rows = 0;
     if (blockIdx.x >= sh.g) return;
-    uint32_t x = sh.start(blockIdx.x);
-    const uint32_t end = sh.start(blockIdx.x + 1);
+    uint32_t x = size ? blockIdx.x : sh.start(blockIdx.x);
+    const uint32_t end = size ? x + 1 : sh.start(blockIdx.x + 1);
     while (x < end) {
-        uint32_t i = 0; // the slot that tile x belongs to
+        uint32_t i = 0; // the slot that tile, or share, x belongs to
         for (uint32_t k = 0; k < c.slots; k += 64) i += (uint32_t)__popcll(__ballot(plan.end[k + lane] <= x));
         const Slot s = slot_of(c, i);
         const uint32_t each = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan.each[i]), base = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan.end[i]) - each * c.heads;
         const uint32_t head = (x - base) / each;
-        int from = (int)(x - base - head * each), blk = 0;
+        int from = (int)(x - base - head * each), blk = 0, to;
         Range r = block_range<QT>(s, 0, a);
-        while (from >= r.cnt) from -= r.cnt, r = block_range<QT>(s, ++blk, a);
-        const int to = min(r.cnt, from + (int)(end - x));
+        const auto length = [&]() { return size ? (r.cnt + (int)size - 1) / (int)size : r.cnt; };
+        int len = length();
+        while (from >= len) from -= len, r = block_range<QT>(s, ++blk, a), len = length();
+        uint32_t w0, w1; // the workgroups that share the pair
+        if (size) {
+            w0 = x - (uint32_t)from, w1 = w0 + (uint32_t)len - 1;
+            const uint32_t k = (uint32_t)from, cnt = (uint32_t)r.cnt;
+            const uint32_t least = cnt / (uint32_t)len, more = cnt - least * (uint32_t)len;
+            from = (int)(k * least + min(k, more)), to = (int)((k + 1) * least + min(k + 1, more));
+        } else {
+            to = min(r.cnt, from + (int)(end - x));
+            w0 = sh.owner(x - (uint32_t)from), w1 = sh.owner(x - (uint32_t)from + (uint32_t)r.cnt - 1);
+        }
         const int M = s.n * group, m0 = blk * 16 * QT;
 
         Attn<TYPE, D, QT, U> A{a, lane};
@@ -438,8 +461,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
         const bool whole = from == 0 && to == r.cnt;
         const uint32_t which = from == 0, slot = blockIdx.x * 2 + which;
         if (!whole && threadIdx.x == 0) {
-            const uint32_t x0 = x - (uint32_t)from;
-            Part p = {(uint32_t)min(16 * QT, M - m0), (uint32_t)s.first, (uint32_t)m0, head, sh.owner(x0), sh.owner(x0 + (uint32_t)r.cnt - 1), {0, 0}};
+            Part p = {(uint32_t)min(16 * QT, M - m0), (uint32_t)s.first, (uint32_t)m0, head, w0, w1, {0, 0}};
             parts[which] = p;
         }
 #pragma unroll
@@ -484,7 +506,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
             }
         }
         __syncthreads();
-        x += (uint32_t)(to - from);
+        x += size ? 1 : (uint32_t)(to - from);
     }
 }
 
@@ -545,7 +567,8 @@ QW_JOIN(1)
 QW_JOIN(2)
 
 // ---------------------------------------------------------------- rows into the cache and out of it
-// The unit that holds token `token` of slot i; null: it has no page.
+// The unit that holds token `token` of slot i and a head; null: it has no page. Head after head lies head_bytes further.
+__device__ __forceinline__ size_t head_bytes(const qwk_kv &c) { return (size_t)c.unit << (c.page_log2 - 4); }
 __device__ __forceinline__ uint8_t *unit_of(const qwk_kv &c, uint32_t i, int token, uint32_t head) {
     const uint64_t at = (uint64_t)i * c.max_pages + ((uint32_t)token >> c.page_log2);
     const uint32_t page = token < 0 ? 0xffffffffu : words(c.table)[at], pu = c.page_log2 - 4;
@@ -559,97 +582,286 @@ template <int TYPE> __device__ __forceinline__ uint32_t place(uint32_t D, bool v
 __device__ __forceinline__ uint32_t place_scale(uint32_t D, bool values, uint32_t t, uint32_t v) { return (values ? 33 : 16) * D + (t / 4 * (D / 32) + v / 32) * 8 + t % 4 * 2; }
 
 __device__ __forceinline__ float half_of(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
-__device__ __forceinline__ uint16_t half_bits(double x) { return __builtin_bit_cast(uint16_t, (_Float16)(float)x); }
+// x to binary16, rounded once. By way of 32 bits, which goes wrong only where those lie between two halves, or below the normal ones: there with the last bit set for what
+// was rounded off. (As one conversion it is some 35 instructions a value: 47 us for 4096 rows of 40 heads, bound by them.)
+__device__ __forceinline__ uint16_t half_bits(double x) {
+    float f = (float)x;
+    uint32_t b = __builtin_bit_cast(uint32_t, f);
+    asm("" : "+v"(b));
+    if (__builtin_expect((b & 0x1fff) == 0x1000 || (b & 0x7fffffff) < 0x38800000, 0)) {
+        const double off = x - (double)f;
+        if (off != 0 && !(b & 1)) b += (off > 0) == (f > 0) ? 1 : -1;
+    }
+    return __builtin_bit_cast(uint16_t, (_Float16)__builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ uint32_t row16_max(uint32_t x) { // over a row of sixteen lanes
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false)); // row_ror:1, 2, 4, 8
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));
+}
+// Q8_0 of 32 values, two a lane: d = max |x| / 127 in binary16, a code is round(x / d). Both operands of the division have 11 bits, so that its rounding to
+// 24 never crosses a border between two codes. Returns the codes, a byte each, the first below.
+__device__ __forceinline__ uint32_t quantise(uint32_t x, uint16_t &scale) {
+    const uint32_t b = row16_max(max(x & 0x7fffu, x >> 16 & 0x7fffu)); // magnitudes order as their bits; NaN above infinity
+    const bool fine = b < 0x7c00;
+    const _Float16 d = fine ? (_Float16)(half_of((uint16_t)b) / 127.f) : (_Float16)__builtin_nanf("");
+    scale = __builtin_bit_cast(uint16_t, d);
+    const float f = fine ? (float)d : 0.f, inv = f > 0 ? 1.f / f : 0.f;
+    const auto code = [&](uint16_t h) { // x / d to the nearest whole number, ties to even: the product with 1 / d is at most one off, what it leaves of x is exact
+        const float v = half_of(h), q = rintf(v * inv), left = __builtin_fmaf(-q, f, v);
+        const float more = __builtin_fmaf(2.f, __builtin_fabsf(left), -f); // (0 where x lies between two codes)
+        const float to = q + (left > 0 ? 1.f : -1.f);
+        const float r = more > 0 || (more == 0 && ((int)q & 1)) ? to : q;
+        return (uint32_t)(int)(f > 0 ? fminf(fmaxf(r, -127.f), 127.f) : 0.f) & 0xff;
+    };
+    return code((uint16_t)x) | code((uint16_t)(x >> 16)) << 8;
+}
 
-// Values lane + 64 c of one head of one row: x, turned by the row's angles (cos, sin of value lane + 64 c) where they are below rot
-__device__ __forceinline__ void put(const qwk_kv &c, int type, uint8_t *unit, bool values, uint32_t t, const uint16_t *x, uint32_t lane) {
-    const uint32_t D = c.dim;
-    for (uint32_t k = 0; k < D / 64; k++) {
-        const uint32_t v = lane + 64 * k;
-        if (type == F16) {
-            *(uint16_t *)(unit + place<F16>(D, values, t, v)) = x[k];
-            continue;
+// `waves` waves of a row take its heads in turn, queries, then keys, then values, two values a lane (four where a head has more than 128). Sines and cosines of the positions, in 64
+// bits, are made once a wave. Four tokens of values lie beside one another in the cache: the wave of the first one's row stores all of them that are rows of this step. Sixteen rows
+// in a row go to one XCD, whose cache then holds whole lines of their units.
+template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(const qwk_kv_write_args &a) {
+    constexpr uint32_t N = 4, W = QW_WG_KV / 64; // heads in hand at once
+    const qwk_kv &c = a.c;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), D = c.dim, n16 = QW_UNIT / W * a.waves, even = gridDim.x / (8 * n16) * (8 * n16);
+    const uint32_t wg = blockIdx.x < even ? (blockIdx.x / (8 * n16) * 8 + blockIdx.x % 8) * n16 + blockIdx.x / 8 % n16 : blockIdx.x;
+    const uint32_t row = (wg * W + wave) / a.waves, mine = (wg * W + wave) % a.waves, step = a.waves;
+    const uint32_t qk = a.q_heads + c.heads, half = a.rot / 2;
+    if (row >= c.rows) return;
+    __shared__ double turns[W][64 * C][2]; // of a wave: cosine and sine of every pair
+    auto &turn = turns[wave];
+    uint32_t d[C]; // pairs of values
+    const bool odd = !a.adjacent && half % 2; // partners of two neighbours are no neighbours
+    uint32_t py[C][2];                        // partners
+#pragma unroll
+    for (uint32_t k = 0; k < C; k++) {
+        d[k] = lane + 64 * k;
+#pragma unroll
+        for (uint32_t e = 0; e < 2; e++) {
+            const uint32_t v = 2 * d[k] + e;
+            py[k][e] = v >= a.rot ? v : a.adjacent ? v ^ 1 : v >= half ? v - half : v + half;
         }
-        // d = max |x| / 127 of 32 values, in binary16; a code is round(x / d). Both operands of the division have 11 bits, so that its rounding to
-        // 24 never crosses a border between two codes.
-        const float f = half_of(x[k]);
-        uint32_t b = x[k] & 0x7fff; // magnitudes order as their bits; NaN above infinity
-        for (int o = 1; o < 32; o <<= 1) b = max(b, (uint32_t)__shfl_xor((int)b, o));
-        const bool fine = b < 0x7c00;
-        const _Float16 d = fine ? (_Float16)(half_of((uint16_t)b) / 127.f) : (_Float16)__builtin_nanf("");
-        const float q = fine && (float)d > 0 ? fminf(fmaxf(rintf(f / (float)d), -127.f), 127.f) : 0.f;
-        *(int8_t *)(unit + place<Q8>(D, values, t, v)) = (int8_t)q;
-        if (lane % 32 == 0) *(_Float16 *)(unit + place_scale(D, values, t, v)) = d;
+    }
+    uint32_t x[N][C], y[N][C], nx[N][C], ny[N][C];
+    const auto load = [&](uint32_t h0, uint32_t (&x)[N][C], uint32_t (&y)[N][C]) {
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++) {
+            const uint32_t h = h0 + n * step;
+            if (h >= qk) break;
+            const uint16_t *src = h < a.q_heads ? a.q + (size_t)row * a.q_stride + (size_t)h * D : a.k + (size_t)row * a.k_stride + (size_t)(h - a.q_heads) * D;
+#pragma unroll
+            for (uint32_t k = 0; k < C; k++) {
+                if (2 * d[k] >= D) continue;
+                x[n][k] = ((const uint32_t *)src)[d[k]];
+                if (a.adjacent) y[n][k] = x[n][k] >> 16 | x[n][k] << 16;
+                else if (!odd) y[n][k] = ((const uint32_t *)src)[py[k][0] / 2];
+                else y[n][k] = src[py[k][0]] | (uint32_t)src[py[k][1]] << 16;
+            }
+        }
+    };
+    load(mine, nx, ny); // (the first heads' values on their way while the row's place and angles are found)
+    uint32_t i;
+    Slot s;
+    if (!slot_find(c, row, i, s)) return;
+    const int token = s.len - s.n + (int)row - s.first;
+    const uint32_t t = (uint32_t)token % 16;
+    double cs[C][2], sn[C][2]; // of each value: result = x cs + partner sn
+    if (mine < qk) {
+#pragma unroll
+        for (uint32_t k = 0; k < C; k++) {
+            const uint32_t p = d[k];
+            if (p >= half) continue;
+            const int32_t pos = a.pos[(size_t)row * a.axes + (a.axes == 1 || p < a.pairs0 ? 0 : p < a.pairs0 + a.pairs1 ? 1 : 2)];
+            double sine, cosine;
+            sincos((double)pos * a.freq[p], &sine, &cosine);
+            turn[p][0] = cosine, turn[p][1] = sine;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // (the wave's own LDS: in order)
+#pragma unroll
+        for (uint32_t k = 0; k < C; k++)
+#pragma unroll
+            for (uint32_t e = 0; e < 2; e++) {
+                const uint32_t v = 2 * d[k] + e;
+                cs[k][e] = 1, sn[k][e] = 0;
+                if (v >= a.rot) continue;
+                const bool second = a.adjacent ? e : v >= half;
+                const uint32_t p = a.adjacent ? v / 2 : second ? v - half : v;
+                cs[k][e] = turn[p][0], sn[k][e] = second ? turn[p][1] : -turn[p][1];
+            }
+    }
+    uint8_t *const unit0 = unit_of(c, i, token, 0);
+#pragma unroll 1
+    for (uint32_t h0 = mine; h0 < qk; h0 += N * step) {
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+            for (uint32_t k = 0; k < C; k++) x[n][k] = nx[n][k], y[n][k] = ny[n][k];
+        load(h0 + N * step, nx, ny);
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++) {
+            const uint32_t h = h0 + n * step;
+            if (h >= qk) break;
+            uint8_t *unit = h < a.q_heads || !unit0 ? nullptr : unit0 + (h - a.q_heads) * head_bytes(c);
+#pragma unroll
+            for (uint32_t k = 0; k < C; k++) {
+                if (2 * d[k] >= D) continue;
+                uint32_t r = x[n][k];
+                if (2 * d[k] < a.rot) // (an even number: both values turn or neither)
+                    r = half_bits((double)half_of((uint16_t)r) * cs[k][0] + (double)half_of((uint16_t)y[n][k]) * sn[k][0]) |
+                        (uint32_t)half_bits((double)half_of((uint16_t)(r >> 16)) * cs[k][1] + (double)half_of((uint16_t)(y[n][k] >> 16)) * sn[k][1]) << 16;
+                if (h < a.q_heads) ((uint32_t *)(a.q_out + (size_t)row * a.qo_stride + (size_t)h * D))[d[k]] = r;
+                else if (TYPE == F16) {
+                    if (unit) *(uint32_t *)(unit + place<F16>(D, false, t, 2 * d[k])) = r;
+                } else {
+                    uint16_t scale;
+                    const uint32_t codes = quantise(r, scale);
+                    if (unit) *(uint16_t *)(unit + place<Q8>(D, false, t, 2 * d[k])) = (uint16_t)codes;
+                    if (unit && lane % 16 == 0) *(uint16_t *)(unit + place_scale(D, false, t, 2 * d[k])) = scale;
+                }
+            }
+        }
+    }
+    if (!unit0 || (t % 4 && (int)row != s.first)) return;
+    const uint32_t rows = min(4 - t % 4, (uint32_t)(s.first + s.n) - row);
+    for (uint32_t h = (mine < qk ? mine + (qk - mine + step - 1) / step * step : mine); h < qk + c.heads; h += step) {
+        uint8_t *const unit = unit0 + (h - qk) * head_bytes(c);
+        uint32_t x[4][C];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+            for (uint32_t k = 0; k < C; k++) x[j][k] = j < rows && 2 * d[k] < D ? ((const uint32_t *)(a.v + (size_t)(row + j) * a.v_stride + (size_t)(h - qk) * D))[d[k]] : 0;
+#pragma unroll
+        for (uint32_t k = 0; k < C; k++) {
+            if (2 * d[k] >= D) continue;
+            if (TYPE == F16) {
+                uint16_t *to = (uint16_t *)(unit + place<F16>(D, true, t, 2 * d[k])); // the second value four tokens on
+                if (rows == 4)
+                    *(uint4_t *)to = uint4_t{(x[0][k] & 0xffff) | x[1][k] << 16, (x[2][k] & 0xffff) | x[3][k] << 16, x[0][k] >> 16 | (x[1][k] & 0xffff0000u), x[2][k] >> 16 | (x[3][k] & 0xffff0000u)};
+                else
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++)
+                        if (j < rows) to[j] = (uint16_t)x[j][k], to[4 + j] = (uint16_t)(x[j][k] >> 16);
+            } else {
+                uint32_t q[4];
+                uint16_t scale[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) q[j] = quantise(x[j][k], scale[j]);
+                uint8_t *to = unit + place<Q8>(D, true, t, 2 * d[k]), *scales = unit + place_scale(D, true, t, 2 * d[k]);
+                if (rows == 4) {
+                    *(uint2_t *)to = uint2_t{(q[0] & 0xff) | (q[1] & 0xff) << 8 | (q[2] & 0xff) << 16 | q[3] << 24, q[0] >> 8 | (q[1] & 0xff00) | (q[2] & 0xff00) << 8 | (q[3] & 0xff00) << 16};
+                    if (lane % 16 == 0) *(uint2_t *)scales = uint2_t{scale[0] | (uint32_t)scale[1] << 16, scale[2] | (uint32_t)scale[3] << 16};
+                } else
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++)
+                        if (j < rows) {
+                            to[j] = (uint8_t)q[j], to[4 + j] = (uint8_t)(q[j] >> 8);
+                            if (lane % 16 == 0) *(uint16_t *)(scales + 2 * j) = scale[j];
+                        }
+            }
+        }
     }
 }
+extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f1_c1(qwk_kv_write_args a) { kv_write_body<F16, 1>(a); }
+extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f1_c2(qwk_kv_write_args a) { kv_write_body<F16, 2>(a); }
+extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f8_c1(qwk_kv_write_args a) { kv_write_body<Q8, 1>(a); }
+extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f8_c2(qwk_kv_write_args a) { kv_write_body<Q8, 2>(a); }
 
-// A wave a head of a row: queries, then keys, then values
-__device__ __forceinline__ void kv_write_body(const qwk_kv_write_args &a, int type) {
-    const qwk_kv &c = a.c;
-    const uint32_t lane = threadIdx.x & 63, D = c.dim, row = blockIdx.x, h = __builtin_amdgcn_readfirstlane(blockIdx.y * (QW_WG_KV / 64) + (threadIdx.x >> 6));
-    if (h >= a.q_heads + 2 * c.heads) return;
-    const bool isq = h < a.q_heads, isv = h >= a.q_heads + c.heads;
-    const uint32_t head = isq ? h : isv ? h - a.q_heads - c.heads : h - a.q_heads;
-    uint32_t i;
-    Slot s;
-    if (!slot_find(c, row, i, s)) return;
-    const int token = s.len - s.n + (int)row - s.first;
-    uint8_t *unit = isq ? nullptr : unit_of(c, i, token, head);
-    if (!isq && !unit) return;
-    const uint16_t *src = isq ? a.q + (size_t)row * a.q_stride : isv ? a.v + (size_t)row * a.v_stride : a.k + (size_t)row * a.k_stride;
-    src += (size_t)head * D;
-    uint16_t x[4], y[4];
-    const uint32_t half = a.rot / 2;
-#pragma unroll
-    for (uint32_t k = 0; k < 4; k++)
-        if (k < D / 64) {
-            const uint32_t v = lane + 64 * k;
-            x[k] = src[v];
-            y[k] = isv || v >= a.rot ? 0 : src[a.adjacent ? v ^ 1 : v < half ? v + half : v - half];
-        }
-#pragma unroll
-    for (uint32_t k = 0; k < 4; k++)
-        if (k < D / 64) {
-            const uint32_t v = lane + 64 * k;
-            if (isv || v >= a.rot) continue;
-            const uint32_t p = a.adjacent ? v / 2 : v % half;
-            const bool second = a.adjacent ? v & 1 : v >= half;
-            const int32_t pos = a.pos[(size_t)row * a.axes + (a.axes == 1 || p < a.pairs0 ? 0 : p < a.pairs0 + a.pairs1 ? 1 : 2)];
-            double sn, cs;
-            sincos((double)pos * a.freq[p], &sn, &cs);
-            x[k] = half_bits((double)half_of(x[k]) * cs + (second ? sn : -sn) * (double)half_of(y[k]));
-        }
-    if (isq) {
-#pragma unroll
-        for (uint32_t k = 0; k < 4; k++)
-            if (k < D / 64) a.q_out[(size_t)row * a.qo_stride + (size_t)head * D + lane + 64 * k] = x[k];
-    } else put(c, type, unit, isv, (uint32_t)token % 16, x, lane);
-}
-extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f1(qwk_kv_write_args a) { kv_write_body(a, F16); }
-extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f8(qwk_kv_write_args a) { kv_write_body(a, Q8); }
-
-// A wave a head of a row, keys and values
+// A wave a unit of a slot's rows, a head, and keys or values: it takes the unit as it lies, 16 bytes a lane, and deals it out to the rows. Bound by the rows out.
 template <int TYPE> __device__ __forceinline__ void kv_read_body(const qwk_kv_read_args &a) {
     const qwk_kv &c = a.c;
-    const uint32_t lane = threadIdx.x & 63, D = c.dim, row = blockIdx.x, head = __builtin_amdgcn_readfirstlane(blockIdx.y * (QW_WG_KV / 64) + (threadIdx.x >> 6));
-    if (head >= c.heads) return;
-    uint32_t i;
-    Slot s;
-    if (!slot_find(c, row, i, s)) return;
-    const int token = s.len - s.n + (int)row - s.first;
-    const uint8_t *unit = unit_of(c, i, token, head);
-    const uint32_t t = (uint32_t)token % 16;
-    for (uint32_t k = 0; k < 2 * (D / 64); k++) {
-        const bool values = k >= D / 64;
-        const uint32_t v = lane + 64 * (values ? k - D / 64 : k);
-        uint16_t *dst = values ? a.v + (size_t)row * a.v_stride : a.k + (size_t)row * a.k_stride;
-        if (!unit) { // (no page: nothing is held)
-            dst[(size_t)head * D + v] = 0;
-            continue;
+    const uint32_t lane = threadIdx.x & 63, D = c.dim, task = __builtin_amdgcn_readfirstlane(blockIdx.x * (QW_WG_KV / 64) + (threadIdx.x >> 6));
+    // which slot's, by the units of those before it
+    const uint32_t un = task / (2 * c.heads), head = (task - un * 2 * c.heads) / 2;
+    const bool values = task & 1;
+    uint32_t before = 0, i = 0, skip = 0;
+    bool found = false;
+#pragma unroll 1
+    for (uint32_t k = 0; k < c.slots && !found; k += 64) {
+        const Slot s = slot_of(c, min(k + lane, c.slots - 1));
+        const int from = max(0, s.len - s.n);
+        const uint32_t units = k + lane < c.slots && s.n > 0 && s.len > 0 ? (uint32_t)((s.len - 1) / 16 - from / 16 + 1) : s.n > 0 && k + lane < c.slots ? 1 : 0;
+        const uint32_t end = before + wave_scan(units);
+        const u64 past = __ballot(end <= un);
+        found = past != ~0ull;
+        const uint32_t at = found ? (uint32_t)__builtin_ctzll(~past) : 63;
+        i = k + at, skip = un - ((uint32_t)__builtin_amdgcn_readlane((int)end, at) - (uint32_t)__builtin_amdgcn_readlane((int)units, at));
+        before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+    }
+    if (!found || i >= c.slots) return;
+    const Slot s = slot_of(c, i);
+    const int t0 = (max(0, s.len - s.n) / 16 + (int)skip) * 16; // the unit's first token; row of token x: x - (len - n) + first
+    const int lift = s.first - (s.len - s.n), lo = s.len - s.n, hi = s.len;
+    uint16_t *const rows = (values ? a.v : a.k) + (size_t)head * D;
+    const size_t stride = values ? a.v_stride : a.k_stride;
+    if (skip == 0) // rows before the slot's first token hold nothing
+        for (int x = lo; x < 0 && x < hi; x++)
+            for (uint32_t v = lane; v < D; v += 64) rows[(size_t)(x + lift) * stride + v] = 0;
+    const uint8_t *u = unit_of(c, i, t0, head);
+    const auto in = [&](int x) { return x >= lo && x < hi; };
+    constexpr uint32_t N = TYPE == F16 ? 8 : 4; // of 1024 bytes, in hand at once: all there are
+    const uint32_t all = TYPE == F16 ? D / 32 : D / 64;
+    if (!values) {
+        const int x = t0 + (int)(lane & 15);
+        uint16_t *to = rows + (size_t)(x + lift) * stride + (lane >> 4) * 8;
+        for (uint32_t b0 = 0; b0 < all; b0 += N) {
+            uint4_t k[N];
+            uint16_t f[N][2];
+#pragma unroll
+            for (uint32_t n = 0; n < N; n++) {
+                const uint32_t b = b0 + n;
+                if (b >= all) break;
+                k[n] = u ? *(const uint4_t *)(u + b * 1024 + lane * 16) : uint4_t{0, 0, 0, 0}; // (no page: nothing is held)
+                if (TYPE == Q8)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; h++) f[n][h] = u ? *(const uint16_t *)(u + 16 * D + ((lane & 15) / 4 * (D / 32) + 2 * b + h) * 8 + (lane & 3) * 2) : 0;
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < N; n++) {
+                const uint32_t b = b0 + n;
+                if (b >= all || !in(x)) break;
+                if (TYPE == F16) *(uint4_t *)(to + b * 32) = k[n];
+                else
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const half4_t c0 = codes(h ? k[n].z : k[n].x), c1 = codes(h ? k[n].w : k[n].y);
+                        half8_t r;
+                        for (int j = 0; j < 4; j++) r[j] = (_Float16)((float)c0[j] * half_of(f[n][h])), r[4 + j] = (_Float16)((float)c1[j] * half_of(f[n][h]));
+                        *(half8_t *)(to + b * 64 + h * 32) = r;
+                    }
+            }
         }
-        const uint8_t *p = unit + place<TYPE>(D, values, t, v);
-        dst[(size_t)head * D + v] = TYPE == F16 ? *(const uint16_t *)p
-                                                : __builtin_bit_cast(uint16_t, (_Float16)((float)*(const int8_t *)p * (float)*(const _Float16 *)(unit + place_scale(D, values, t, v))));
+        return;
+    }
+    const int x = t0 + (int)(lane >> 4) * 4;
+    uint16_t *to = rows + (size_t)(x + lift) * stride + (lane & 15) * 2;
+    for (uint32_t b0 = 0; b0 < all; b0 += N) {
+        uint4_t v[N], f[N];
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++) {
+            const uint32_t b = b0 + n;
+            if (b >= all) break;
+            v[n] = u ? *(const uint4_t *)(u + (TYPE == F16 ? 32 : 17) * D + b * 1024 + lane * 16) : uint4_t{0, 0, 0, 0};
+            if (TYPE == Q8) f[n] = u ? *(const uint4_t *)(u + 33 * D + ((lane >> 4) * (D / 32) + 2 * b) * 8) : uint4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++) {
+            const uint32_t b = b0 + n;
+            if (b >= all) break;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (!in(x + j)) continue;
+                if (TYPE == F16) {
+                    const uint32_t p = j & 2 ? v[n].y : v[n].x, q = j & 2 ? v[n].w : v[n].z;
+                    *(uint32_t *)(to + (size_t)j * stride + b * 32) = j & 1 ? p >> 16 | (q & 0xffff0000u) : (p & 0xffff) | q << 16;
+                } else
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float g = (float)__builtin_bit_cast(half4_t, h ? uint2_t{f[n].z, f[n].w} : uint2_t{f[n].x, f[n].y})[j];
+                        *(half2_t *)(to + (size_t)j * stride + b * 64 + h * 32) = half2_t{(_Float16)((float)codes(h ? v[n].z : v[n].x)[j] * g), (_Float16)((float)codes(h ? v[n].w : v[n].y)[j] * g)};
+                    }
+            }
+        }
     }
 }
 extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_read_f1(qwk_kv_read_args a) { kv_read_body<F16>(a); }

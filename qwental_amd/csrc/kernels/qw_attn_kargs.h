@@ -36,7 +36,7 @@ typedef struct {
     uint16_t *q_out;
     const double *freq;
     const int32_t *pos;
-    uint32_t q_stride, qo_stride, k_stride, v_stride, q_heads, rot, axes, pairs0, pairs1, adjacent;
+    uint32_t q_stride, qo_stride, k_stride, v_stride, q_heads, rot, axes, pairs0, pairs1, adjacent, waves; /* waves: of a row */
 } qwk_kv_write_args;
 
 typedef struct {
