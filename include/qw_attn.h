@@ -16,7 +16,7 @@
  *                                 [4][D/32][4 t], values [D/64][4][16][2][2][4 t] int8 (value 64 a + 32 b + 2 c + d at [a][.][c][b][d]), scales
  *                                 of the values [4][D/32][4 t]; scales are binary16, one for 32 values of a token
  * with t = 4 [first of the 4s] + [last of the 4s]. It is the order in which the matrix instructions take them. Q8_0 of 32 values x: d = max |x| / 127 rounded
- * to binary16, codes round(x / d) (0 where d is 0); 32 values of which one is not finite are held as NaN.
+ * to binary16 (at most 515.5, so that a value held stays in that type's range), codes round(x / d) up to 127 (0 where d is 0); 32 values of which one is not finite are held as NaN.
  *
  * A step. Slot i (a conversation) has rows first[i] .. first[i + 1) of the step's `rows`, and, those included, len[i] tokens: its row j
  * is token len[i] - n + j, n = first[i + 1] - first[i]. Token t lies in page table[i][t / page]. first, len and table are read on the device

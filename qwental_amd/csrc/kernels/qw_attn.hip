@@ -75,23 +75,21 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) { // sums over the lan
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
     return x;
 }
-// Tiles (size 0) or shares of up to `size` tiles of all slots, a lane a slot. Every wave makes it and writes it down for itself (all the same, where it is the same LDS): no barrier.
+// Shares of up to `size` tiles (per = 1 / size) that a block of so many tiles is cut into; per 0: its tiles. Only so exact as it has to be: whoever asks for a block gets the same.
+__device__ __forceinline__ int shares_in(int cnt, float per) { return per > 0 ? min((int)((float)(cnt - 1) * per) + 1, cnt) : cnt; }
+// Shares, or tiles, of all slots, a lane a slot. Every wave makes it and writes it down for itself (all the same, where it is the same LDS): no barrier.
 struct Plan { uint32_t each[QW_KV_SLOTS_MAX], end[QW_KV_SLOTS_MAX]; }; // of one of the slot's heads; of all slots up to and with this one
-template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, uint32_t size, uint32_t *pairs) { // returns the whole
+template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, const Slot &first, float per, uint32_t *pairs) { // returns the whole; first: the lane's slot
     const uint32_t lane = threadIdx.x & 63;
     uint32_t T = 0, P = 0;
 #pragma unroll 1
     for (uint32_t k = 0; k < a.c.slots; k += 64) {
         const uint32_t i = k + lane;
         uint32_t each = 0;
-        Slot s = slot_of(a.c, min(i, a.c.slots - 1));
-        asm volatile("" : "+v"(s.n), "+v"(s.len)); // (all three loads at once, not the length's behind a branch on the others)
+        const Slot s = k ? slot_of(a.c, min(i, a.c.slots - 1)) : first;
         const int nb = i < a.c.slots ? blocks_of<QT>(s, a) : 0;
 #pragma unroll 1
-        for (int b = 0; b < nb; b++) {
-            const uint32_t cnt = (uint32_t)block_range<QT>(s, b, a).cnt;
-            each += size ? (cnt + size - 1) / size : cnt;
-        }
+        for (int b = 0; b < nb; b++) each += (uint32_t)shares_in(block_range<QT>(s, b, a).cnt, per);
         const uint32_t end = T + wave_scan(each * a.c.heads);
         p.each[i] = each, p.end[i] = end;
         T = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
@@ -156,7 +154,7 @@ template <int D> struct UnitData<Q8, D> {
     }
     __device__ __forceinline__ uint2_t odd() const {
         uint2_t o = {0, 0};
-        const auto full = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+        const auto full = [](uint32_t w) { return ((w & 0x7fff7fffu) + 0x1ff81ff8u) & 0x80008000u; }; // from 516 on, whose products with a code may be more than binary16 holds
 #pragma unroll
         for (int c = 0; c < D / 64; c++) o |= uint2_t{full(s[c].x) | full(s[c].z), full(s[c].y) | full(s[c].w)};
         return o;
@@ -197,9 +195,9 @@ template <int TYPE, int D, int QT, int U> struct Attn {
         }
         return s;
     }
-    // Weights in two parts, binary16 each: together they hold 21 bits, so that the result is as exact as its own rounding. The largest weight is 2^TOP, not 1, so that the
-    // small ones do not end at binary16's 2^-24: many tokens of 2^-25 of the largest's weight count for something together. (Q8_0: a weight is multiplied by a scale of up to 516.)
-    static constexpr float TOP = TYPE == F16 ? 14.f : 6.f;
+    // Weights in two parts, binary16 each: together they hold 21 bits, so that the result is as exact as its own rounding. The largest weight is 2^14, not 1, so that the
+    // small ones do not end at binary16's 2^-24: many tokens of 2^-25 of the largest's weight count for something together.
+    static constexpr float TOP = 14.f;
     __device__ __forceinline__ static void split(const float4_t &p, half4_t &h, half4_t &r) {
         const half2_t h0 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(p[0], p[1])), h1 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(p[2], p[3]));
         float d[4];
@@ -216,14 +214,17 @@ template <int TYPE, int D, int QT, int U> struct Attn {
     // key0: first token of the step's first unit; bad: units without a page; edge: some query does not see all of the step's tokens
     __device__ __forceinline__ void softmax(int key0, uint32_t bad, bool edge, float4_t (&p)[QT][U]) {
         const float neg = -__builtin_inff();
-        if (edge)
+        if (edge) {
+            int first = key0 + (int)(lane >> 4) * 4;
+            asm volatile("" : "+v"(first)); // (or the comparisons are made in every step, ahead of the branch)
 #pragma unroll
             for (int t = 0; t < QT; t++)
 #pragma unroll
                 for (int i = 0; i < U; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        if (hidden(t, key0 + i * 16 + (int)(lane >> 4) * 4 + j, bad, i)) p[t][i][j] = neg;
+                        if (hidden(t, first + i * 16 + j, bad, i)) p[t][i][j] = neg;
+        }
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             float top = neg;
@@ -255,28 +256,41 @@ template <int TYPE, int D, int QT, int U> struct Attn {
 #pragma unroll
         for (int i = 0; i < U; i++) {
             half4_t h[QT], r[QT];
-            if constexpr (TYPE == F16)
 #pragma unroll
-                for (int t = 0; t < QT; t++) split(p[t][i], h[t], r[t]);
+            for (int t = 0; t < QT; t++) split(p[t][i], h[t], r[t]);
 #pragma unroll
             for (int b = 0; b < D / 32; b++) {
-                const half4_t v0 = values(i, b, 0), v1 = values(i, b, 1);
-                if constexpr (TYPE == Q8) {
-                    const half4_t f = V[i].scales(b); // a token's scale belongs to its weight
+                if constexpr (TYPE == F16) {
+                    const half4_t v0 = values(i, b, 0), v1 = values(i, b, 1);
 #pragma unroll
                     for (int t = 0; t < QT; t++) {
-                        float4_t w;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) w[k] = p[t][i][k] * (float)f[k];
-                        split(w, h[t], r[t]);
+                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, h[t], acc[t][b][0], 0, 0, 0);
+                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, h[t], acc[t][b][1], 0, 0, 0);
                     }
-                }
 #pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, h[t], acc[t][b][0], 0, 0, 0);
-                    acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, h[t], acc[t][b][1], 0, 0, 0);
-                    acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, r[t], acc[t][b][0], 0, 0, 0);
-                    acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, r[t], acc[t][b][1], 0, 0, 0);
+                    for (int t = 0; t < QT; t++) {
+                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, r[t], acc[t][b][0], 0, 0, 0);
+                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, r[t], acc[t][b][1], 0, 0, 0);
+                    }
+                } else {
+                    // A value, code times scale, has 18 bits: in two parts too, exactly, side by side in one operand of 8 against (h, h) and (r, r). (The scale multiplied into every weight instead, as the
+                    // scores' is, cost every block of 32 values a split of its weights: 346 vector instructions a step of two blocks of queries of 128 values, now 226. One kind of matrix instruction for
+                    // an accumulator: sums that went from 16x16x32 on in 16x16x16 came out wrong here, the compiler leaving too little room between the two.)
+                    const half4_t f = V[i].scales(b), c0 = values(i, b, 0), c1 = values(i, b, 1), v0 = c0 * f, v1 = c1 * f;
+                    const half4_t w0 = __builtin_elementwise_fma(c0, f, -v0), w1 = __builtin_elementwise_fma(c1, f, -v1);
+                    const half8_t a0 = __builtin_shufflevector(v0, w0, 0, 1, 2, 3, 4, 5, 6, 7), a1 = __builtin_shufflevector(v1, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int t = 0; t < QT; t++) {
+                        const half8_t hh = __builtin_shufflevector(h[t], h[t], 0, 1, 2, 3, 4, 5, 6, 7);
+                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hh, acc[t][b][0], 0, 0, 0);
+                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hh, acc[t][b][1], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int t = 0; t < QT; t++) {
+                        const half8_t rr = __builtin_shufflevector(r[t], r[t], 0, 1, 2, 3, 4, 5, 6, 7);
+                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, rr, acc[t][b][0], 0, 0, 0);
+                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, rr, acc[t][b][1], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -336,26 +350,30 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
     Part *parts = (Part *)a.parts + blockIdx.x * 2;
     __shared__ Plan plan;
     // The least size of a share that the grid is enough for: 4 tiles, or a round more than equal shares of everything would have, or two. (To begin once more in another pair costs a
-    // workgroup some 5 us, as much as two rounds.) Otherwise (size 0) shares of the whole line.
-    uint32_t pairs, size = 0;
-    const uint32_t T = make_plan<QT>(plan, a, 0, &pairs);
+    // workgroup some 5 us, as much as two rounds.) Otherwise (per 0) shares of the whole line.
+    Slot mine = slot_of(c, min(lane, c.slots - 1));
+    asm volatile("" : "+v"(mine.n), "+v"(mine.len)); // (all three loads at once, not the length's behind a branch on the others)
+    uint32_t pairs;
+    float per = 0;
+    const uint32_t T = make_plan<QT>(plan, a, mine, 0, &pairs);
     Shares sh = {0, 0, 0};
     if (pairs <= a.grid) {
         const uint32_t least = max(4u, (T + a.grid - 1) / a.grid + 3 & ~3u);
 #pragma unroll 1
-        for (uint32_t k = 0; k < 3 && !size; k++) {
-            sh.g = make_plan<QT>(plan, a, least + 4 * k, nullptr);
-            if (sh.g <= a.grid) size = least + 4 * k;
+        for (uint32_t k = 0; k < 3 && per == 0; k++) {
+            const float x = __builtin_amdgcn_rcpf((float)(least + 4 * k));
+            sh.g = make_plan<QT>(plan, a, mine, x, nullptr);
+            if (sh.g <= a.grid) per = x;
         }
     }
-    if (!size) {
-        if (pairs <= a.grid) make_plan<QT>(plan, a, 0, nullptr);
+    if (per == 0) {
+        if (pairs <= a.grid) make_plan<QT>(plan, a, mine, 0, nullptr);
         sh.g = min(a.grid, T), sh.base = T / max(sh.g, 1u), sh.more = T - sh.base * sh.g;
     }
     if (threadIdx.x < 2) parts[threadIdx.x].rows = 0;
     if (blockIdx.x >= sh.g) return;
-    uint32_t x = size ? blockIdx.x : sh.start(blockIdx.x);
-    const uint32_t end = size ? x + 1 : sh.start(blockIdx.x + 1);
+    uint32_t x = per > 0 ? blockIdx.x : sh.start(blockIdx.x);
+    const uint32_t end = per > 0 ? x + 1 : sh.start(blockIdx.x + 1);
     while (x < end) {
         uint32_t i = 0; // the slot that tile, or share, x belongs to
         for (uint32_t k = 0; k < c.slots; k += 64) i += (uint32_t)__popcll(__ballot(plan.end[k + lane] <= x));
@@ -364,11 +382,10 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
         const uint32_t head = (x - base) / each;
         int from = (int)(x - base - head * each), blk = 0, to;
         Range r = block_range<QT>(s, 0, a);
-        const auto length = [&]() { return size ? (r.cnt + (int)size - 1) / (int)size : r.cnt; };
-        int len = length();
-        while (from >= len) from -= len, r = block_range<QT>(s, ++blk, a), len = length();
+        int len = shares_in(r.cnt, per);
+        while (from >= len) from -= len, r = block_range<QT>(s, ++blk, a), len = shares_in(r.cnt, per);
         uint32_t w0, w1; // the workgroups that share the pair
-        if (size) {
+        if (per > 0) {
             w0 = x - (uint32_t)from, w1 = w0 + (uint32_t)len - 1;
             const uint32_t k = (uint32_t)from, cnt = (uint32_t)r.cnt;
             const uint32_t least = cnt / (uint32_t)len, more = cnt - least * (uint32_t)len;
@@ -398,14 +415,22 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
         const size_t in_page = (size_t)head << pu;
         const uint8_t *u[U];
         uint32_t bad;
+        const uint32_t unit = c.unit, in_mask = (1u << pu) - 1;
+        const uint8_t *const heads = c.cache + in_page * unit;
         const auto find = [&](int key0) {
             bad = 0;
-#pragma unroll
-            for (int k = 0; k < U; k++) {
-                const uint32_t un = (uint32_t)(key0 >> 4) + k, at = un >> pu;
-                uint32_t page = at < c.max_pages ? table[at] : 0xffffffffu;
-                if (page >= c.pages) bad |= 1u << k, page = 0;
-                u[k] = c.cache + page * c.page_bytes + (in_page + (un & ((1u << pu) - 1))) * c.unit;
+            const uint32_t un = (uint32_t)(key0 >> 4);
+            uint32_t at = un >> pu, page = at < c.max_pages ? table[at] : 0xffffffffu;
+            if (page >= c.pages) bad = (1u << U) - 1, page = 0;
+            u[0] = heads + page * c.page_bytes + (un & in_mask) * unit;
+            if (U == 2) {
+                u[U - 1] = u[0] + unit;
+                if (pu == 0) { // (a page is one unit: elsewhere a tile lies in one page)
+                    at++, page = at < c.max_pages ? table[at] : 0xffffffffu;
+                    bad &= 1;
+                    if (page >= c.pages) bad |= 2, page = 0;
+                    u[U - 1] = heads + page * c.page_bytes;
+                }
             }
         };
         const int steps = max(0, (to - from - (int)wave + W - 1) / W) * STEPS;
@@ -506,7 +531,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
             }
         }
         __syncthreads();
-        x += size ? 1 : (uint32_t)(to - from);
+        x += per > 0 ? 1 : (uint32_t)(to - from);
     }
 }
 
@@ -600,12 +625,12 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t x) { // over a row of six
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
     return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));
 }
-// Q8_0 of 32 values, two a lane: d = max |x| / 127 in binary16, a code is round(x / d). Both operands of the division have 11 bits, so that its rounding to
+// Q8_0 of 32 values, two a lane: d = max |x| / 127 in binary16 (at most 515.5: 127 times 516 is more than that holds), a code is round(x / d). Both operands of the division have 11 bits, so that its rounding to
 // 24 never crosses a border between two codes. Returns the codes, a byte each, the first below.
 __device__ __forceinline__ uint32_t quantise(uint32_t x, uint16_t &scale) {
     const uint32_t b = row16_max(max(x & 0x7fffu, x >> 16 & 0x7fffu)); // magnitudes order as their bits; NaN above infinity
     const bool fine = b < 0x7c00;
-    const _Float16 d = fine ? (_Float16)(half_of((uint16_t)b) / 127.f) : (_Float16)__builtin_nanf("");
+    const _Float16 d = fine ? (_Float16)fminf(half_of((uint16_t)b) / 127.f, 515.5f) : (_Float16)__builtin_nanf("");
     scale = __builtin_bit_cast(uint16_t, d);
     const float f = fine ? (float)d : 0.f, inv = f > 0 ? 1.f / f : 0.f;
     const auto code = [&](uint16_t h) { // x / d to the nearest whole number, ties to even: the product with 1 / d is at most one off, what it leaves of x is exact

@@ -31,7 +31,7 @@ def quantised(x):
     b = x.astype(np.float64).reshape(*x.shape[:-1], -1, 32)
     top = np.abs(b).max(-1)
     with np.errstate(invalid="ignore"):
-        d = (top / 127).astype(np.float16)
+        d = np.minimum(top / 127, 515.5).astype(np.float16)  # 127 * 516 is beyond binary16
         d = np.where(np.isfinite(top), d, np.float16(np.nan))
         c = np.where((d > 0)[..., None], np.rint(b / np.where(d > 0, d, 1).astype(np.float64)[..., None]), 0)
     return np.clip(c, -127, 127).astype(np.int8).reshape(x.shape), d
@@ -138,7 +138,7 @@ def attention(cache, step, query, scale, window=0, dead=()):
         p = np.exp(s - s.max(-1, keepdims=True))
         p /= p.sum(-1, keepdims=True)
         out[row] = np.einsum("hgt,thd->hgd", p, v).reshape(Hq, D)
-        floor = len(seen) * p.max(-1, keepdims=True) * (2.0 ** -39 * np.abs(v).max() if cache.kind == F16 else 127 * 2.0 ** -31)
+        floor = len(seen) * p.max(-1, keepdims=True) * 2.0 ** -39 * np.abs(v).max()
         tol[row] = (tolerance(out[row], np.einsum("hgt,thd->hgd", p, np.abs(v)), size, len(seen), D) + floor).reshape(Hq, D)
     return out, tol
 
@@ -147,8 +147,7 @@ def tolerance(o, weight, size, T, D):
     """The result is rounded to binary16 once: half a step, 2^-11 of it, or 2^-25 where binary16 steps are 2^-24. A score is a sum of D products in binary32 (2^-24 a step, D steps at
     most, of at most `size` = scale * sum |q k|), times a scale rounded to 24 bits and log2(e) (two more steps), brought to its weight by a subtraction and an exponential
     (another two steps of the score's size, 2^-22 for the exponential): relative error e of a weight, which enters numerator and denominator. The weights of the second product
-    are held in 22 bits (2^-22), or times a scale in 21; its sums over T tokens run in tiles of 16, each lane's over T / 4 of them at most: T / 4 + 8 steps of 2^-24 of sum p |v|, as do those of the
-    denominator. `weight` = sum p |v|. (The caller adds what the smallest weights lose: half of binary16's last step, 2^-25, where the largest weight is 2^14, each times a value; for
-    Q8_0 where it is 2^6, each times a code of up to 127.)"""
+    are held in 21 bits; its sums over T tokens run in tiles of 16, each lane's over T / 4 of them at most: T / 4 + 8 steps of 2^-24 of sum p |v|, as do those of the
+    denominator. `weight` = sum p |v|. (The caller adds what the smallest weights lose: half of binary16's last step, 2^-25, where the largest weight is 2^14, each times a value.)"""
     e = (D + 6) * 2.0 ** -24 * size + 2.0 ** -22
     return 2.0 ** -11 * np.abs(o.reshape(weight.shape)) + 2.0 ** -25 + weight * (2 * e + 2.0 ** -21 + 2 * (T / 4 + 8) * 2.0 ** -24)
