@@ -22,8 +22,10 @@
  * is token len[i] - n + j, n = first[i + 1] - first[i]. Token t lies in page table[i][t / page]. first, len and table are read on the device
  * when the kernels run, so a captured sequence goes on being right as the slots grow. Rows that belong to no slot are left as they are. What the
  * device finds there cannot be refused any more, and nothing out of bounds is touched for it: a slot whose rows do not lie in the step has
- * none, len counts up to max_pages * page, a page number from `pages` on is no page - its tokens are not written, read back as zeros and not
- * attended to.
+ * none (for qw_attn no slot has any from where first decreases), len counts up to max_pages * page, a page number from `pages` on is no page -
+ * its tokens are not written, read back as zeros and not attended to. Slots may share pages that the step only reads.
+ *
+ * What a call writes lies apart from what it reads (q_out = q excepted): an overlap is refused.
  */
 #pragma once
 #include "gpu.h"
@@ -91,8 +93,8 @@ bool qw_sample(qw_batch *b, int rows, int vocab, int stride, const qw_at *logits
 
 /* A recorder for callers with streams and memory of their own (a framework's tensors, a stream under graph capture): begin, any of the
  * functions above, end. The launches go to `stream` (a hipStream_t of this device; NULL: the default stream), in order, and end returns without
- * waiting; nothing is allocated, copied or synchronised. Buffers have to be device-only: qw_hip_buf_new_device, or views. One
- * recorder at a time per device (NULL + qw_hip_last_error otherwise); qw_hip_stream_end gives it back and launches nothing where a function failed.
+ * waiting; nothing is allocated, copied or synchronised. Buffers have to be device-only: qw_hip_buf_new_device, or views. It holds
+ * 64 launches (qw_attn and qw_sample make two each); a call that finds no room fails. One recorder at a time per device (NULL + qw_hip_last_error otherwise); qw_hip_stream_end gives it back and launches nothing where a function failed.
  * qw_path_gg_moe_noalloc uses the same one. */
 qw_batch *qw_hip_stream_begin(qw_gpu *g, void *stream);
 bool qw_hip_stream_end(qw_batch *b);

@@ -2478,26 +2478,37 @@ static bool kv_rows(qw_batch *b, unsigned index, bool out, const qw_attn_geo *x,
     *str = (uint32_t)stride;
     return true;
 }
-static bool kv_bind(qw_batch *b, qw_attn_geo *x, qwk_kv *c, bool write, qw_span *cache) {
+static qw_span flat(const void *p, size_t bytes) { return (qw_span){p, bytes, bytes, 1}; }
+// What a kernel writes lies apart from what it reads to know where: it would go by what it has just overwritten, out of its bounds too.
+static bool apart_all(qw_batch *b, const qw_span *x, const char *xs, int n, const qw_span *y, const char *const *ys) {
+    for (int i = 0; i < n; i++)
+        if (!apart(b, x, xs, &y[i], ys[i])) return false;
+    return true;
+}
+enum { QW_KV_READS = 4 }; // cache, first, len, table
+static const char *const kv_reads[QW_KV_READS] = {"the cache", "first", "len", "table"};
+static bool kv_bind(qw_batch *b, qw_attn_geo *x, qwk_kv *c, bool write, qw_span (*in)[QW_KV_READS]) {
     if (!bind_bytes(b, QW_ATTN_GEO, x, sizeof *x, "sizes")) return false;
     const size_t bytes = qw_kv_bytes(x->type, x->heads, x->dim, x->page, x->pages);
     if (!bytes) return fail(b, "%s: a cache of type %d, %d heads of %d values, %d pages of %d tokens (types 1 and 8, 1 to %d heads of 64, 128, 192 or 256 values, pages of a power of two from 16 to %d)", b->k->name, x->type,
                             x->heads, x->dim, x->pages, x->page, QW_ATTN_MAX_HEADS, QW_ATTN_MAX_PAGE);
     if (x->slots < 1 || x->slots > QW_KV_MAX_SLOTS || x->rows < 1 || x->rows > QW_KV_MAX_ROWS) return fail(b, "%s: %d slots, %d rows (1 to %d, 1 to %d)", b->k->name, x->slots, x->rows, QW_KV_MAX_SLOTS, QW_KV_MAX_ROWS);
-    if (x->max_pages < 1 || (int64_t)x->max_pages * x->page > INT32_MAX / 2) return fail(b, "%s: %d pages a slot of %d tokens (up to 2^30 tokens)", b->k->name, x->max_pages, x->page);
+    if (x->max_pages < 1 || (int64_t)x->max_pages * x->page > 1 << 30) return fail(b, "%s: %d pages a slot of %d tokens (up to 2^30 tokens)", b->k->name, x->max_pages, x->page);
     *c = (qwk_kv){.slots = (uint32_t)x->slots, .rows = (uint32_t)x->rows, .max_pages = (uint32_t)x->max_pages, .pages = (uint32_t)x->pages, .page_log2 = (uint32_t)__builtin_ctz((unsigned)x->page), .heads = (uint32_t)x->heads,
                   .dim = (uint32_t)x->dim, .unit = (uint32_t)(x->dim * (x->type == 1 ? 64 : 34)), .page_bytes = bytes / (size_t)x->pages};
-    if (!bind_ptr(b, 0, bytes, write, "cache", (void **)&c->cache) || !bind_ptr(b, 1, ((size_t)x->slots + 1) * 4, false, "first", (void **)&c->first) || !bind_ptr(b, 2, (size_t)x->slots * 4, false, "len", (void **)&c->len) ||
-        !bind_ptr(b, 3, (size_t)x->slots * (size_t)x->max_pages * 4, false, "table", (void **)&c->table)) return false;
+    const size_t S = (size_t)x->slots, T = S * (size_t)x->max_pages;
+    if (!bind_ptr(b, 0, bytes, write, "cache", (void **)&c->cache) || !bind_ptr(b, 1, (S + 1) * 4, false, "first", (void **)&c->first) || !bind_ptr(b, 2, S * 4, false, "len", (void **)&c->len) ||
+        !bind_ptr(b, 3, T * 4, false, "table", (void **)&c->table)) return false;
     if ((uintptr_t)c->cache % 16 || (uintptr_t)c->first % 4 || (uintptr_t)c->len % 4 || (uintptr_t)c->table % 4) return fail(b, "%s: cache, first, len and table must be 16- and 4-byte aligned", b->k->name);
-    *cache = (qw_span){(const char *)c->cache, bytes, bytes, 1};
-    return true;
+    const qw_span all[QW_KV_READS] = {flat(c->cache, bytes), flat(c->first, (S + 1) * 4), flat(c->len, S * 4), flat(c->table, T * 4)};
+    memcpy(*in, all, sizeof all);
+    return !write || apart_all(b, &all[0], kv_reads[0], QW_KV_READS - 1, all + 1, kv_reads + 1);
 }
 static bool tr_kv_write(qw_batch *b) {
     qw_attn_geo x;
     qwk_kv_write_args a = {0};
-    qw_span cache, q = {0}, qo = {0}, k, v;
-    if (!kv_bind(b, &x, &a.c, true, &cache)) return false;
+    qw_span in[QW_KV_READS], q = {0}, qo = {0}, k, v, freq = {0}, pos = {0};
+    if (!kv_bind(b, &x, &a.c, true, &in)) return false;
     if (x.q_heads < 0 || x.q_heads > QW_ATTN_MAX_Q_HEADS) return fail(b, "kv_write: %d query heads (0 to %d)", x.q_heads, QW_ATTN_MAX_Q_HEADS);
     if (x.q_heads && (!kv_rows(b, 4, false, &x, x.q_heads, x.stride[0], "q", (uint16_t **)&a.q, &a.q_stride, &q) || !kv_rows(b, 5, true, &x, x.q_heads, x.stride[1], "q_out", &a.q_out, &a.qo_stride, &qo))) return false;
     if (!kv_rows(b, 6, false, &x, x.heads, x.stride[2], "k", (uint16_t **)&a.k, &a.k_stride, &k) || !kv_rows(b, 7, false, &x, x.heads, x.stride[3], "v", (uint16_t **)&a.v, &a.v_stride, &v)) return false;
@@ -2508,11 +2519,13 @@ static bool tr_kv_write(qw_batch *b) {
             return fail(b, "kv_write: %d + %d + %d pairs of values for %d", x.pairs[0], x.pairs[1], x.pairs[2], x.rot);
         if (!bind_ptr(b, 8, (size_t)x.rot / 2 * 8, false, "freq", (void **)&a.freq) || !bind_ptr(b, 9, (size_t)x.rows * (size_t)x.axes * 4, false, "pos", (void **)&a.pos)) return false;
         if ((uintptr_t)a.freq % 8 || (uintptr_t)a.pos % 4) return fail(b, "kv_write: freq and pos must be 8- and 4-byte aligned");
+        freq = flat(a.freq, (size_t)x.rot / 2 * 8), pos = flat(a.pos, (size_t)x.rows * (size_t)x.axes * 4);
     }
     // q_out may be q: a wave has read a head before it writes it
     if (qo.p && !(qo.p == q.p && qo.stride == q.stride) && !apart(b, &qo, "q_out", &q, "q")) return false;
-    if (!apart(b, &qo, "q_out", &k, "k") || !apart(b, &qo, "q_out", &v, "v") || !apart(b, &qo, "q_out", &cache, "the cache") || !apart(b, &q, "q", &cache, "the cache") || !apart(b, &k, "k", &cache, "the cache") ||
-        !apart(b, &v, "v", &cache, "the cache")) return false;
+    const qw_span read[] = {k, v, freq, pos, q};
+    static const char *const reads[] = {"k", "v", "freq", "pos", "q"};
+    if (!apart_all(b, &qo, "q_out", 4, read, reads) || !apart_all(b, &qo, "q_out", QW_KV_READS, in, kv_reads) || !apart_all(b, &in[0], "the cache", 5, read, reads)) return false;
     a.q_heads = (uint32_t)x.q_heads, a.rot = (uint32_t)x.rot, a.axes = (uint32_t)x.axes, a.pairs0 = (uint32_t)x.pairs[0], a.pairs1 = (uint32_t)x.pairs[1], a.adjacent = x.adjacent != 0;
     // A wave a head while that makes no more than eight waves for each SIMD of the device, then several heads a wave: what a row costs before its first head is then shared
     const unsigned heads = (unsigned)(x.q_heads + 2 * x.heads), waves = (unsigned)b->g->ncu * 32 / (unsigned)x.rows;
@@ -2523,10 +2536,10 @@ static bool tr_kv_write(qw_batch *b) {
 static bool tr_kv_read(qw_batch *b) {
     qw_attn_geo x;
     qwk_kv_read_args a = {0};
-    qw_span cache, k, v;
-    if (!kv_bind(b, &x, &a.c, false, &cache)) return false;
+    qw_span in[QW_KV_READS], k, v;
+    if (!kv_bind(b, &x, &a.c, false, &in)) return false;
     if (!kv_rows(b, 6, true, &x, x.heads, x.stride[2], "k", &a.k, &a.k_stride, &k) || !kv_rows(b, 7, true, &x, x.heads, x.stride[3], "v", &a.v, &a.v_stride, &v)) return false;
-    if (!apart(b, &k, "k", &v, "v") || !apart(b, &k, "k", &cache, "the cache") || !apart(b, &v, "v", &cache, "the cache")) return false;
+    if (!apart(b, &k, "k", &v, "v") || !apart_all(b, &k, "k", QW_KV_READS, in, kv_reads) || !apart_all(b, &v, "v", QW_KV_READS, in, kv_reads)) return false;
     // a wave a unit and head, for keys and for values: 16 rows a unit, and for every slot one begun and one ended within a unit
     const unsigned units = (unsigned)x.rows / QW_UNIT + 2 * umin((unsigned)x.slots, (unsigned)x.rows);
     return add_launch(b, x.type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", cdiv(units * 2 * (unsigned)x.heads, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
@@ -2546,8 +2559,8 @@ static bool tr_attn(qw_batch *b) {
                                                {{"qwk_attn_f8_d64_q1", "qwk_attn_f8_d64_q2"}, {"qwk_attn_f8_d128_q1", "qwk_attn_f8_d128_q2"}, {"qwk_attn_f8_d192_q1", "qwk_attn_f8_d192_q2"}, {"qwk_attn_f8_d256_q1", "qwk_attn_f8_d256_q2"}}};
     qw_attn_geo x;
     qwk_attn_args a = {0};
-    qw_span cache, q, out, ws;
-    if (!kv_bind(b, &x, &a.c, false, &cache)) return false;
+    qw_span in[QW_KV_READS], q, out;
+    if (!kv_bind(b, &x, &a.c, false, &in)) return false;
     if (x.q_heads < 1 || x.q_heads > QW_ATTN_MAX_Q_HEADS || x.q_heads % x.heads) return fail(b, "attn_paged: %d query heads for %d of keys (a multiple, up to %d)", x.q_heads, x.heads, QW_ATTN_MAX_Q_HEADS);
     // tiles of all pairs are counted in 32 bits
     if ((((uint64_t)x.rows * (uint64_t)x.q_heads + 15) / 16 + (uint64_t)x.slots * (uint64_t)x.heads) * ((uint64_t)x.max_pages * (uint64_t)x.page / QW_ATTN_TILE + 2) > INT32_MAX)
@@ -2557,9 +2570,9 @@ static bool tr_attn(qw_batch *b) {
     const size_t need = qw_attn_ws_bytes(b->g, x.dim);
     if (!bind_ptr(b, 6, need, true, "workspace", (void **)&a.part)) return false;
     if ((uintptr_t)a.part % 16) return fail(b, "attn_paged: the workspace must be 16-byte aligned");
-    ws = (qw_span){(const char *)a.part, need, need, 1};
-    if (!apart(b, &out, "out", &q, "q") || !apart(b, &out, "out", &cache, "the cache") || !apart(b, &ws, "the workspace", &q, "q") || !apart(b, &ws, "the workspace", &out, "out") || !apart(b, &ws, "the workspace", &cache, "the cache"))
-        return false;
+    const qw_span ws = flat(a.part, need);
+    if (!apart(b, &out, "out", &q, "q") || !apart(b, &ws, "the workspace", &q, "q") || !apart(b, &ws, "the workspace", &out, "out") || !apart_all(b, &out, "out", QW_KV_READS, in, kv_reads) ||
+        !apart_all(b, &ws, "the workspace", QW_KV_READS, in, kv_reads)) return false;
     a.group = (uint32_t)(x.q_heads / x.heads), a.window = (uint32_t)x.window, a.grid = attn_grid(b->g);
     a.scale = (x.scale > 0 ? x.scale : 1 / sqrtf((float)x.dim)) * 1.44269504f;
     // rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode
@@ -2592,6 +2605,10 @@ static bool tr_sample(qw_batch *b) {
     void *ws;
     if (!bind_ptr(b, 5, qw_sample_ws_bytes(b->g, x.rows, x.vocab), true, "workspace", &ws)) return false;
     if ((uintptr_t)ws % 16) return fail(b, "sample_rows: the workspace must be 16-byte aligned");
+    const qw_span all[] = {flat(a.ids, R * 4), flat(a.probs, R * 4), flat(ws, qw_sample_ws_bytes(b->g, x.rows, x.vocab)), flat(a.logits, ((R - 1) * (size_t)stride + (size_t)x.vocab) * 4), flat(a.p, R * sizeof(qwk_sample_row)), flat(a.u, R * 4)};
+    static const char *const what[] = {"ids", "probs", "the workspace", "logits", "parameters", "u"};
+    for (int i = 0; i < 3; i++) // the outputs, with all that come behind them
+        if (!apart_all(b, &all[i], what[i], 5 - i, all + i + 1, what + i + 1)) return false;
     const size_t n = R * a.tiles; // the tiles' tokens first: the others' sizes keep 16 bytes for none of them
     a.order = ws, a.start = a.order + n * QW_SAMPLE_TILE, a.weight = (uint64_t *)(a.start + n * QW_SAMPLE_STARTS), a.head = a.weight + n * QW_SAMPLE_BINS;
     if (!add_launch(b, "qwk_sample_bins", (unsigned)x.rows, QW_WG_SAMPLE_BINS, &a, sizeof a)) return false;

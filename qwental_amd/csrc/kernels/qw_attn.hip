@@ -38,7 +38,7 @@ __device__ __forceinline__ Slot slot_of(const qwk_kv &c, uint32_t i) {
     const uint32_t room = c.max_pages << c.page_log2; // (up to 2^30)
     Slot s;
     s.first = (int)a;
-    s.n = (a <= b) & (b <= c.rows) ? (int)(b - a) : 0; // what is no row of the step is not touched
+    s.n = a > b ? -1 : b <= c.rows ? (int)(b - a) : 0; // what is no row of the step is not touched
     s.len = (int)min(l, room);
     return s;
 }
@@ -82,12 +82,15 @@ struct Plan { uint32_t each[QW_KV_SLOTS_MAX], end[QW_KV_SLOTS_MAX]; }; // of one
 template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, const Slot &first, float per, uint32_t *pairs) { // returns the whole; first: the lane's slot
     const uint32_t lane = threadIdx.x & 63;
     uint32_t T = 0, P = 0;
+    bool wrong = false; // first[] has decreased: slots could have more rows together than there are, and more tiles than are counted in 32 bits. From there on they have none
 #pragma unroll 1
     for (uint32_t k = 0; k < a.c.slots; k += 64) {
         const uint32_t i = k + lane;
         uint32_t each = 0;
         const Slot s = k ? slot_of(a.c, min(i, a.c.slots - 1)) : first;
-        const int nb = i < a.c.slots ? blocks_of<QT>(s, a) : 0;
+        const u64 back = __ballot(s.n < 0);
+        const int nb = i < a.c.slots && !wrong && !(back << 63 - lane) ? blocks_of<QT>(s, a) : 0;
+        wrong |= back != 0;
 #pragma unroll 1
         for (int b = 0; b < nb; b++) each += (uint32_t)shares_in(block_range<QT>(s, b, a).cnt, per);
         const uint32_t end = T + wave_scan(each * a.c.heads);
@@ -544,6 +547,7 @@ template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args 
     const float neg = -__builtin_inff();
     const Part p = ((const Part *)a.parts)[blockIdx.x * 2 + blockIdx.y];
     if (!p.rows) return;
+    if (p.w1 >= a.grid || p.head >= a.c.heads || p.row0 + (uint32_t)by(a.by_group, (int)(p.m0 + p.rows - 1)) >= a.c.rows) return; // (of another call that was given this workspace at the same time)
     const uint32_t np = p.w1 - p.w0 + 1, all = p.rows * D4, k = blockIdx.x - p.w0;
     const uint32_t o1 = (k + 1) * all / np;
     // one with what another left
