@@ -77,10 +77,13 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) { // sums over the lan
 }
 // Shares of up to `size` tiles (per = 1 / size) that a block of so many tiles is cut into; per 0: its tiles. Only so exact as it has to be: whoever asks for a block gets the same.
 __device__ __forceinline__ int shares_in(int cnt, float per) { return per > 0 ? min((int)((float)(cnt - 1) * per) + 1, cnt) : cnt; }
-// Shares, or tiles, of all slots, a lane a slot. Every wave makes it and writes it down for itself (all the same, where it is the same LDS): no barrier.
+// Shares, or tiles, of all slots, a lane a slot. Every wave works it out for itself. Only the plan that is gone by in the end is written down: all waves then write the same, and none needs
+// a barrier; one of those before it, written by a wave that is behind, would lie in the place of what another already reads.
 struct Plan { uint32_t each[QW_KV_SLOTS_MAX], end[QW_KV_SLOTS_MAX]; }; // of one of the slot's heads; of all slots up to and with this one
-template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const qwk_attn_args &a, const Slot &first, float per, uint32_t *pairs) { // returns the whole; first: the lane's slot
+struct Count { uint32_t all, pairs, each, end; }; // of all slots; of the lane's, among the first 64
+template <int QT, bool WRITE> __device__ __forceinline__ Count make_plan(Plan &p, const qwk_attn_args &a, const Slot &first, float per) { // first: the lane's slot
     const uint32_t lane = threadIdx.x & 63;
+    Count r = {0, 0, 0, 0};
     uint32_t T = 0, P = 0;
     bool wrong = false; // first[] has decreased: slots could have more rows together than there are, and more tiles than are counted in 32 bits. From there on they have none
 #pragma unroll 1
@@ -94,12 +97,13 @@ template <int QT> __device__ __forceinline__ uint32_t make_plan(Plan &p, const q
 #pragma unroll 1
         for (int b = 0; b < nb; b++) each += (uint32_t)shares_in(block_range<QT>(s, b, a).cnt, per);
         const uint32_t end = T + wave_scan(each * a.c.heads);
-        p.each[i] = each, p.end[i] = end;
+        if (WRITE) p.each[i] = each, p.end[i] = end;
+        if (k == 0) r.each = each, r.end = end;
         T = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
-        if (pairs) P += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)nb), 63);
+        P += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)nb), 63);
     }
-    if (pairs) *pairs = P * a.c.heads;
-    return T;
+    r.all = T, r.pairs = P * a.c.heads;
+    return r;
 }
 // Shares along the line of all tiles: workgroup w of g takes the next T / g tiles, the first T % g of them one more.
 struct Shares {
@@ -356,21 +360,22 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
     // workgroup some 5 us, as much as two rounds.) Otherwise (per 0) shares of the whole line.
     Slot mine = slot_of(c, min(lane, c.slots - 1));
     asm volatile("" : "+v"(mine.n), "+v"(mine.len)); // (all three loads at once, not the length's behind a branch on the others)
-    uint32_t pairs;
     float per = 0;
-    const uint32_t T = make_plan<QT>(plan, a, mine, 0, &pairs);
+    Count count = make_plan<QT, false>(plan, a, mine, 0);
+    const uint32_t T = count.all;
     Shares sh = {0, 0, 0};
-    if (pairs <= a.grid) {
+    if (count.pairs <= a.grid) {
         const uint32_t least = max(4u, (T + a.grid - 1) / a.grid + 3 & ~3u);
 #pragma unroll 1
         for (uint32_t k = 0; k < 3 && per == 0; k++) {
             const float x = __builtin_amdgcn_rcpf((float)(least + 4 * k));
-            sh.g = make_plan<QT>(plan, a, mine, x, nullptr);
-            if (sh.g <= a.grid) per = x;
+            count = make_plan<QT, false>(plan, a, mine, x);
+            if ((sh.g = count.all) <= a.grid) per = x;
         }
     }
+    if (c.slots > 64 || (per == 0 && count.all != T)) make_plan<QT, true>(plan, a, mine, per);
+    else plan.each[lane] = count.each, plan.end[lane] = count.end;
     if (per == 0) {
-        if (pairs <= a.grid) make_plan<QT>(plan, a, mine, 0, nullptr);
         sh.g = min(a.grid, T), sh.base = T / max(sh.g, 1u), sh.more = T - sh.base * sh.g;
     }
     if (threadIdx.x < 2) parts[threadIdx.x].rows = 0;
