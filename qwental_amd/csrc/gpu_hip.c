@@ -229,7 +229,8 @@ static const qw_wg_rule wg_rules[] = {
     {"qwk_moe_prep", QW_WG_PREP, 0, 0},
     {"qwk_hc_up", QW_WG_HC_UP, 0, 0},
     {"qwk_attn_join", QW_WG_JOIN, 0, 0},
-    {"qwk_attn_", QW_WG_ATTN, 0, 0},
+    {"qwk_attn_w8_", 512, 0, 0},
+    {"qwk_attn_w4_", 256, 0, 0},
     {"qwk_kv_", QW_WG_KV, 0, 0},
     {"qwk_sample_bins", QW_WG_SAMPLE_BINS, 0, 0},
     {"qwk_sample", QW_WG_SAMPLE, 0, 0},
@@ -2544,8 +2545,8 @@ static bool tr_kv_read(qw_batch *b) {
     const unsigned units = (unsigned)x.rows / QW_UNIT + 2 * umin((unsigned)x.slots, (unsigned)x.rows);
     return add_launch(b, x.type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", cdiv(units * 2 * (unsigned)x.heads, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
 }
-// Two workgroups a compute unit; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
-static unsigned attn_grid(const qw_gpu *g) { return 2 * (unsigned)g->ncu; }
+// A workgroup a compute unit: eight waves, or four where a wave has all of a SIMD's registers; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
+static unsigned attn_grid(const qw_gpu *g) { return (unsigned)g->ncu; }
 static size_t attn_part_bytes(const qw_gpu *g, int dim, unsigned qt) { return (size_t)attn_grid(g) * 2 * 16 * qt * (size_t)dim * 4; }
 size_t qw_attn_ws_bytes(const qw_gpu *g, int dim) { return !g || dim < 64 || dim > 256 || dim % 64 ? 0 : attn_part_bytes(g, dim, 2) + attn_part_bytes(g, 2, 2) + (size_t)attn_grid(g) * 2 * QW_ATTN_PART; }
 // Division by d for dividends below 2^31: with 2^l >= d the least such power, mul = floor(2^(31 + l) / d) + 1 is off by less than 2^l / 2^31 of a step for each of them.
@@ -2555,8 +2556,8 @@ static qwk_div div_of(uint32_t d) {
     return d <= 1 ? (qwk_div){0, 0} : (qwk_div){(uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1};
 }
 static bool tr_attn(qw_batch *b) {
-    static const char *const names[2][4][2] = {{{"qwk_attn_f1_d64_q1", "qwk_attn_f1_d64_q2"}, {"qwk_attn_f1_d128_q1", "qwk_attn_f1_d128_q2"}, {"qwk_attn_f1_d192_q1", "qwk_attn_f1_d192_q2"}, {"qwk_attn_f1_d256_q1", "qwk_attn_f1_d256_q2"}},
-                                               {{"qwk_attn_f8_d64_q1", "qwk_attn_f8_d64_q2"}, {"qwk_attn_f8_d128_q1", "qwk_attn_f8_d128_q2"}, {"qwk_attn_f8_d192_q1", "qwk_attn_f8_d192_q2"}, {"qwk_attn_f8_d256_q1", "qwk_attn_f8_d256_q2"}}};
+    static const char *const names[2][4][2] = {{{"qwk_attn_w8_f1_d64_q1", "qwk_attn_w8_f1_d64_q2"}, {"qwk_attn_w8_f1_d128_q1", "qwk_attn_w8_f1_d128_q2"}, {"qwk_attn_w8_f1_d192_q1", "qwk_attn_w4_f1_d192_q2"}, {"qwk_attn_w8_f1_d256_q1", "qwk_attn_w4_f1_d256_q2"}},
+                                               {{"qwk_attn_w8_f8_d64_q1", "qwk_attn_w8_f8_d64_q2"}, {"qwk_attn_w8_f8_d128_q1", "qwk_attn_w8_f8_d128_q2"}, {"qwk_attn_w8_f8_d192_q1", "qwk_attn_w4_f8_d192_q2"}, {"qwk_attn_w8_f8_d256_q1", "qwk_attn_w4_f8_d256_q2"}}};
     qw_attn_geo x;
     qwk_attn_args a = {0};
     qw_span in[QW_KV_READS], q, out;
@@ -2573,14 +2574,15 @@ static bool tr_attn(qw_batch *b) {
     const qw_span ws = flat(a.part, need);
     if (!apart(b, &out, "out", &q, "q") || !apart(b, &ws, "the workspace", &q, "q") || !apart(b, &ws, "the workspace", &out, "out") || !apart_all(b, &out, "out", QW_KV_READS, in, kv_reads) ||
         !apart_all(b, &ws, "the workspace", QW_KV_READS, in, kv_reads)) return false;
-    a.group = (uint32_t)(x.q_heads / x.heads), a.window = (uint32_t)x.window, a.grid = attn_grid(b->g);
+    a.group = (uint32_t)(x.q_heads / x.heads), a.window = x.window > 1 << 30 ? 0 : (uint32_t)x.window, a.grid = attn_grid(b->g);
     a.scale = (x.scale > 0 ? x.scale : 1 / sqrtf((float)x.dim)) * 1.44269504f;
     // rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode
     const unsigned qt = cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
     a.ml = a.part + attn_part_bytes(b->g, x.dim, 2) / 4;
     a.parts = a.ml + attn_part_bytes(b->g, 2, 2) / 4;
     a.by_group = div_of(a.group);
-    if (!add_launch(b, names[x.type == 8][x.dim / 64 - 1][qt - 1], a.grid, QW_WG_ATTN, &a, sizeof a)) return false;
+    const char *name = names[x.type == 8][x.dim / 64 - 1][qt - 1];
+    if (!add_launch(b, name, a.grid, name[strlen("qwk_attn_w")] == '8' ? 512 : 256, &a, sizeof a)) return false;
     if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", a.grid, QW_WG_JOIN, &a, sizeof a)) return false;
     b->l[b->nl - 1].gy = 2; // of the pair that a workgroup went on with, and of the one that it began
     return true;

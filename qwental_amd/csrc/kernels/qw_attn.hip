@@ -347,17 +347,17 @@ struct Part {
 };
 static_assert(sizeof(Part) == QW_ATTN_PART, "");
 
-template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
-    constexpr int U = D <= 128 ? 2 : 1, W = QW_WG_ATTN / 64, LD = D + 4, STEPS = 2 / U; // U: units a wave has in hand; a tile is two
-    __shared__ float4_t so[W][16][LD / 4];
-    __shared__ float sm[W][16], sl[W][16];
+template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
+    constexpr int U = D <= 128 ? 2 : 1, LD = D + 4, STEPS = 2 / U; // U: units a wave has in hand; a tile is two
+    __shared__ float4_t so[W][16 * QT][LD / 4];
+    __shared__ float sm[W][16 * QT], sl[W][16 * QT];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const qwk_kv &c = a.c;
     const int group = (int)a.group, window = (int)a.window;
     Part *parts = (Part *)a.parts + blockIdx.x * 2;
     __shared__ Plan plan;
-    // The least size of a share that the grid is enough for: 4 tiles, or a round more than equal shares of everything would have, or two. (To begin once more in another pair costs a
-    // workgroup some 5 us, as much as two rounds.) Otherwise (per 0) shares of the whole line.
+    // The least size of a share that the grid is enough for: 4 tiles, or what equal shares of everything would have, or up to 16 more. (To begin once more in another pair costs a
+    // workgroup some 5 us, as much as two rounds of its waves.) Otherwise (per 0) shares of the whole line.
     Slot mine = slot_of(c, min(lane, c.slots - 1));
     asm volatile("" : "+v"(mine.n), "+v"(mine.len)); // (all three loads at once, not the length's behind a branch on the others)
     float per = 0;
@@ -365,9 +365,9 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
     const uint32_t T = count.all;
     Shares sh = {0, 0, 0};
     if (count.pairs <= a.grid) {
-        const uint32_t least = max(4u, (T + a.grid - 1) / a.grid + 3 & ~3u);
+        const uint32_t equal = max(4u, (T + a.grid - 1) / a.grid), least = equal <= W ? equal : equal + 3 & ~3u;
 #pragma unroll 1
-        for (uint32_t k = 0; k < 3 && per == 0; k++) {
+        for (uint32_t k = 0; k < 5 && per == 0; k++) {
             const float x = __builtin_amdgcn_rcpf((float)(least + 4 * k));
             count = make_plan<QT, false>(plan, a, mine, x);
             if ((sh.g = count.all) <= a.grid) per = x;
@@ -499,43 +499,44 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
         }
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-            if (m0 + t * 16 >= M) break;
             float l = A.l[t];
             l += __shfl_xor(l, 16);
             l += __shfl_xor(l, 32);
-            __syncthreads();
-            if (lane < 16) sm[wave][lane] = A.m[t], sl[wave][lane] = l;
+            if (lane < 16) sm[wave][t * 16 + lane] = A.m[t], sl[wave][t * 16 + lane] = l;
 #pragma unroll
             for (int b = 0; b < D / 32; b++) {
                 const float4_t u0 = A.acc[t][b][0], u1 = A.acc[t][b][1];
-                float4_t *o = &so[wave][lane & 15][b * 8 + (lane >> 4) * 2];
+                float4_t *o = &so[wave][t * 16 + (lane & 15)][b * 8 + (lane >> 4) * 2];
                 o[0] = float4_t{u0[0], u1[0], u0[1], u1[1]}, o[1] = float4_t{u0[2], u1[2], u0[3], u1[3]};
             }
-            __syncthreads();
-            const int row = threadIdx.x / 16, mr = m0 + t * 16 + row;
-            if (mr < M) {
-                float top = -__builtin_inff(), sum = 0, f[W];
-                for (int w = 0; w < W; w++) top = fmaxf(top, sm[w][row]);
-                for (int w = 0; w < W; w++) {
-                    f[w] = sm[w][row] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm[w][row] - top);
-                    sum += sl[w][row] * f[w];
-                }
-                const int j = by(a.by_group, mr);
-                uint16_t *out = a.out + (size_t)(s.first + j) * a.out_stride + ((size_t)head * group + (mr - j * group)) * D;
-                const size_t left = (size_t)slot * 16 * QT + t * 16 + row;
-                if (!whole && threadIdx.x % 16 == 0) a.ml[left * 2] = top, a.ml[left * 2 + 1] = sum;
-                const float inv = top == -__builtin_inff() ? 0.f : 1.f / sum; // a row that sees nothing: zeros
+        }
+        __syncthreads();
+        constexpr int PER_ROW = W * 64 / (16 * QT); // threads
+        const int row = (int)threadIdx.x / PER_ROW, mr = m0 + row;
+        if (mr < M) {
+            float top = -__builtin_inff(), sum = 0, f[W];
 #pragma unroll
-                for (int v = 0; v < D / 64; v++) {
-                    const int at4 = v * 16 + (int)(threadIdx.x % 16);
-                    float4_t o = {0, 0, 0, 0};
-                    for (int w = 0; w < W; w++) o += so[w][row][at4] * f[w];
-                    if (whole) {
-                        half4_t h;
-                        for (int k = 0; k < 4; k++) h[k] = (_Float16)(top == -__builtin_inff() ? 0.f : o[k] * inv);
-                        *(half4_t *)(out + at4 * 4) = h;
-                    } else *(float4_t *)(a.part + left * D + at4 * 4) = o;
-                }
+            for (int w = 0; w < W; w++) top = fmaxf(top, f[w] = sm[w][row]);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                f[w] = f[w] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(f[w] - top);
+                sum += sl[w][row] * f[w];
+            }
+            const int j = by(a.by_group, mr);
+            uint16_t *out = a.out + (size_t)(s.first + j) * a.out_stride + ((size_t)head * group + (mr - j * group)) * D;
+            const size_t left = (size_t)slot * 16 * QT + row;
+            if (!whole && threadIdx.x % PER_ROW == 0) a.ml[left * 2] = top, a.ml[left * 2 + 1] = sum;
+            const float inv = top == -__builtin_inff() ? 0.f : 1.f / sum; // a row that sees nothing: zeros
+#pragma unroll
+            for (int at4 = (int)threadIdx.x % PER_ROW; at4 < D / 4; at4 += PER_ROW) {
+                float4_t o = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < W; w++) o += so[w][row][at4] * f[w];
+                if (whole) {
+                    half4_t h;
+                    for (int k = 0; k < 4; k++) h[k] = (_Float16)(top == -__builtin_inff() ? 0.f : o[k] * inv);
+                    *(half4_t *)(out + at4 * 4) = h;
+                } else *(float4_t *)(a.part + left * D + at4 * 4) = o;
             }
         }
         __syncthreads();
@@ -589,13 +590,12 @@ template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args 
     }
 }
 
-#define QW_ATTN(TYPE, D, QT, PER) \
-    extern "C" __global__ __launch_bounds__(QW_WG_ATTN, PER) void qwk_attn_f##TYPE##_d##D##_q##QT(qwk_attn_args a) { attn_body<TYPE, D, QT>(a); }
-#define QW_ATTN_D(D, P1, P2) QW_ATTN(1, D, 1, P1) QW_ATTN(8, D, 1, P1) QW_ATTN(1, D, 2, P2) QW_ATTN(8, D, 2, P2)
-QW_ATTN_D(64, 2, 2)
-QW_ATTN_D(128, 2, 2)
-QW_ATTN_D(192, 2, 1)
-QW_ATTN_D(256, 2, 1)
+#define QW_ATTN(W, TYPE, D, QT, PER) \
+    extern "C" __global__ __launch_bounds__(W * 64, PER) void qwk_attn_w##W##_f##TYPE##_d##D##_q##QT(qwk_attn_args a) { attn_body<TYPE, D, QT, W>(a); }
+QW_ATTN(8, 1, 64, 1, 2) QW_ATTN(8, 8, 64, 1, 2) QW_ATTN(8, 1, 64, 2, 2) QW_ATTN(8, 8, 64, 2, 2)
+QW_ATTN(8, 1, 128, 1, 2) QW_ATTN(8, 8, 128, 1, 2) QW_ATTN(8, 1, 128, 2, 2) QW_ATTN(8, 8, 128, 2, 2)
+QW_ATTN(8, 1, 192, 1, 2) QW_ATTN(8, 8, 192, 1, 2) QW_ATTN(4, 1, 192, 2, 1) QW_ATTN(4, 8, 192, 2, 1)
+QW_ATTN(8, 1, 256, 1, 2) QW_ATTN(8, 8, 256, 1, 2) QW_ATTN(4, 1, 256, 2, 1) QW_ATTN(4, 8, 256, 2, 1)
 #define QW_JOIN(QT) extern "C" __global__ __launch_bounds__(QW_WG_JOIN) void qwk_attn_join_q##QT(qwk_attn_args a) { join_body<QT>(a); }
 QW_JOIN(1)
 QW_JOIN(2)
@@ -624,7 +624,7 @@ __device__ __forceinline__ uint16_t half_bits(double x) {
     asm("" : "+v"(b));
     if (__builtin_expect((b & 0x1fff) == 0x1000 || (b & 0x7fffffff) < 0x38800000, 0)) {
         const double off = x - (double)f;
-        if (off != 0 && !(b & 1)) b += (off > 0) == (f > 0) ? 1 : -1;
+        if (off != 0 && !(b & 1)) b += (off > 0) == !(b >> 31) ? 1 : -1; // (by its sign bit: f may be 0)
     }
     return __builtin_bit_cast(uint16_t, (_Float16)__builtin_bit_cast(float, b));
 }

@@ -273,3 +273,28 @@ def test_strides_and_offsets(gpu, dev):
     o = out[0].read(offset=48, dtype=np.float16).reshape(6, -1)
     fine = np.isfinite(want[:5]).all((1, 2)) & (np.abs(want[:5]).max((1, 2)) < 60000)
     assert (np.abs(o[:5, :Hq * D].reshape(5, Hq, D) - want[:5])[fine] <= tol[:5][fine]).all() and not o[:, Hq * D:].any() and not o[5].any()
+
+
+@pytest.mark.parametrize("window", [(1 << 30) - 1, 1 << 30, (1 << 31) - 1])
+def test_windows_larger_than_everything(gpu, dev, window):
+    rng = np.random.default_rng(23)
+    s = Step(rng, [5, 1, 40], [2, 70, 9], 16)  # rows before their slot's first token too
+    c = filled(rng, Q8, 2, 64, 16, s)
+    got = [check(dev, gpu, np.random.default_rng(1), Q8, 2, 8, 64, 16, s, window=w, c=c) for w in (window, 0)]
+    assert np.array_equal(got[0].view(np.uint16), got[1].view(np.uint16))
+
+
+@pytest.mark.parametrize("freq", [1e-300, 1e-42, 1e-20])
+def test_angles_near_zero(gpu, dev, freq):
+    """Products far below what 32 bits hold: zeros, of either sign."""
+    rng = np.random.default_rng(29)
+    s = Step(rng, [4], [4], 16)
+    c = Cache(F16, 1, 64, 16, s.pages, rng=rng)
+    x = rows(rng, 4, 1, 64)
+    x[..., :32] = 0
+    x[1, :, 32:] = -0.0
+    pos = np.array([[1], [2], [-3], [4]], np.int32)
+    out = dev.new(x.nbytes)
+    xb = dev.up(x)
+    dev.run(q.KvWrite(dev.cache(c), dev.step(s), 1, xb, out, xb, xb, q.Rope(64, [32], dev.up(np.full(32, freq)), dev.up(pos))))
+    assert np.array_equal(out.read(dtype=np.float16).reshape(x.shape), turned(x, pos, np.full(32, freq), [32], False))
