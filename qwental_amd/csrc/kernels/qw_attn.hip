@@ -260,45 +260,47 @@ template <int TYPE, int D, int QT, int U> struct Attn {
         }
     }
     __device__ __forceinline__ void weigh(const float4_t (&p)[QT][U]) {
+        half4_t h[QT][U], r[QT][U];
 #pragma unroll
-        for (int i = 0; i < U; i++) {
-            half4_t h[QT], r[QT];
+        for (int t = 0; t < QT; t++)
 #pragma unroll
-            for (int t = 0; t < QT; t++) split(p[t][i], h[t], r[t]);
+            for (int i = 0; i < U; i++) split(p[t][i], h[t][i], r[t][i]);
+        if constexpr (TYPE == F16) {
 #pragma unroll
-            for (int b = 0; b < D / 32; b++) {
-                if constexpr (TYPE == F16) {
+            for (int i = 0; i < U; i++)
+#pragma unroll
+                for (int b = 0; b < D / 32; b++) {
                     const half4_t v0 = values(i, b, 0), v1 = values(i, b, 1);
 #pragma unroll
                     for (int t = 0; t < QT; t++) {
-                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, h[t], acc[t][b][0], 0, 0, 0);
-                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, h[t], acc[t][b][1], 0, 0, 0);
+                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, h[t][i], acc[t][b][0], 0, 0, 0);
+                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, h[t][i], acc[t][b][1], 0, 0, 0);
                     }
 #pragma unroll
                     for (int t = 0; t < QT; t++) {
-                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, r[t], acc[t][b][0], 0, 0, 0);
-                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, r[t], acc[t][b][1], 0, 0, 0);
-                    }
-                } else {
-                    // A value, code times scale, has 18 bits: in two parts too, exactly, side by side in one operand of 8 against (h, h) and (r, r). (The scale multiplied into every weight instead, as the
-                    // scores' is, cost every block of 32 values a split of its weights: 346 vector instructions a step of two blocks of queries of 128 values, now 226. One kind of matrix instruction for
-                    // an accumulator: sums that went from 16x16x32 on in 16x16x16 came out wrong here, the compiler leaving too little room between the two.)
-                    const half4_t f = V[i].scales(b), c0 = values(i, b, 0), c1 = values(i, b, 1), v0 = c0 * f, v1 = c1 * f;
-                    const half4_t w0 = __builtin_elementwise_fma(c0, f, -v0), w1 = __builtin_elementwise_fma(c1, f, -v1);
-                    const half8_t a0 = __builtin_shufflevector(v0, w0, 0, 1, 2, 3, 4, 5, 6, 7), a1 = __builtin_shufflevector(v1, w1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int t = 0; t < QT; t++) {
-                        const half8_t hh = __builtin_shufflevector(h[t], h[t], 0, 1, 2, 3, 4, 5, 6, 7);
-                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hh, acc[t][b][0], 0, 0, 0);
-                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hh, acc[t][b][1], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int t = 0; t < QT; t++) {
-                        const half8_t rr = __builtin_shufflevector(r[t], r[t], 0, 1, 2, 3, 4, 5, 6, 7);
-                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, rr, acc[t][b][0], 0, 0, 0);
-                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, rr, acc[t][b][1], 0, 0, 0);
+                        acc[t][b][0] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, r[t][i], acc[t][b][0], 0, 0, 0);
+                        acc[t][b][1] = __builtin_amdgcn_mfma_f32_16x16x16f16(v1, r[t][i], acc[t][b][1], 0, 0, 0);
                     }
                 }
+        } else {
+            // Values are code times scale rounded to binary16, as they are read back. An operand of 8 takes the tokens of two units side by side, against both's first parts and then both's
+            // second; of one unit, the same tokens twice, against both parts. (The scale multiplied into every weight instead, as the scores' is, costs every block of 32 values a split of its weights. One kind
+            // of matrix instruction for an accumulator: sums that went from 16x16x32 on in 16x16x16 came out wrong here, the compiler leaving too little room between the two.)
+            const auto eight = [](half4_t x, half4_t y) { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); };
+#pragma unroll
+            for (int b = 0; b < D / 32; b++) {
+                half8_t v[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) v[c] = eight(values(0, b, c) * V[0].scales(b), values(U - 1, b, c) * V[U - 1].scales(b));
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) acc[t][b][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], eight(h[t][0], U == 2 ? h[t][1] : r[t][0]), acc[t][b][c], 0, 0, 0);
+                if (U == 2)
+#pragma unroll
+                    for (int t = 0; t < QT; t++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) acc[t][b][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], eight(r[t][0], r[t][U - 1]), acc[t][b][c], 0, 0, 0);
             }
         }
     }

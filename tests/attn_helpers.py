@@ -132,6 +132,8 @@ def attention(cache, step, query, scale, window=0, dead=()):
         if not seen:
             continue
         k, v = cache.get(step.table, slot, seen)
+        with np.errstate(over="ignore"):
+            v = v.astype(np.float16).astype(np.float64)  # as they are read back
         qr = query[row].astype(np.float64).reshape(cache.heads, G, D)
         s = np.einsum("hgd,thd->hgt", qr, k) * scale
         size = (np.einsum("hgd,thd->hgt", np.abs(qr), np.abs(k)) * scale).max(-1, keepdims=True)
