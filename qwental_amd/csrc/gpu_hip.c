@@ -2580,7 +2580,7 @@ static bool tr_attn(qw_batch *b) {
     const unsigned qt = cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
     a.ml = a.part + attn_part_bytes(b->g, x.dim, 2) / 4;
     a.parts = a.ml + attn_part_bytes(b->g, 2, 2) / 4;
-    a.by_group = div_of(a.group);
+    a.by_group = div_of(a.group), a.by_grid = div_of(a.grid);
     const char *name = names[x.type == 8][x.dim / 64 - 1][qt - 1];
     if (!add_launch(b, name, a.grid, name[strlen("qwk_attn_w")] == '8' ? 512 : 256, &a, sizeof a)) return false;
     if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", a.grid, QW_WG_JOIN, &a, sizeof a)) return false;

@@ -55,6 +55,9 @@ __device__ __forceinline__ bool slot_find(const qwk_kv &c, uint32_t row, uint32_
 }
 __device__ __forceinline__ int by(qwk_div d, int x) { return d.mul ? (int)(__umulhi((uint32_t)x, d.mul) >> d.shift) : x; } // x / d, 0 <= x < 2^31
 
+// Waves meet over LDS alone: what they have on its way from or to memory is not waited for.
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 struct Range { int t0, cnt; }; // a block's first tile, and how many (at least one: an empty one still gives its rows their zeros)
 template <int QT> __device__ __forceinline__ Range block_range(const Slot &s, int b, const qwk_attn_args &a) {
     const int M = s.n * (int)a.group, j0 = by(a.by_group, b * 16 * QT), j1 = by(a.by_group, min((b + 1) * 16 * QT, M) - 1);
@@ -367,7 +370,7 @@ template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_b
     const uint32_t T = count.all;
     Shares sh = {0, 0, 0};
     if (count.pairs <= a.grid) {
-        const uint32_t equal = max(4u, (T + a.grid - 1) / a.grid), least = equal <= W ? equal : equal + 3 & ~3u;
+        const uint32_t equal = max(4u, (uint32_t)by(a.by_grid, (int)(T + a.grid - 1))), least = equal <= W ? equal : equal + 3 & ~3u;
 #pragma unroll 1
         for (uint32_t k = 0; k < 5 && per == 0; k++) {
             const float x = __builtin_amdgcn_rcpf((float)(least + 4 * k));
@@ -387,9 +390,11 @@ template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_b
     while (x < end) {
         uint32_t i = 0; // the slot that tile, or share, x belongs to
         for (uint32_t k = 0; k < c.slots; k += 64) i += (uint32_t)__popcll(__ballot(plan.end[k + lane] <= x));
-        const Slot s = slot_of(c, i);
+        const Slot s = i < 64 ? Slot{__builtin_amdgcn_readlane(mine.n, (int)i), __builtin_amdgcn_readlane(mine.len, (int)i), __builtin_amdgcn_readlane(mine.first, (int)i)} : slot_of(c, i);
         const uint32_t each = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan.each[i]), base = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan.end[i]) - each * c.heads;
-        const uint32_t head = (x - base) / each;
+        uint32_t head = (uint32_t)((float)(x - base) * __builtin_amdgcn_rcpf((float)each)); // (at most 256: one off at most)
+        if (head * each > x - base) head--;
+        if (x - base - head * each >= each) head++;
         int from = (int)(x - base - head * each), blk = 0, to;
         Range r = block_range<QT>(s, 0, a);
         int len = shares_in(r.cnt, per);
@@ -397,9 +402,9 @@ template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_b
         uint32_t w0, w1; // the workgroups that share the pair
         if (per > 0) {
             w0 = x - (uint32_t)from, w1 = w0 + (uint32_t)len - 1;
-            const uint32_t k = (uint32_t)from, cnt = (uint32_t)r.cnt;
-            const uint32_t least = cnt / (uint32_t)len, more = cnt - least * (uint32_t)len;
-            from = (int)(k * least + min(k, more)), to = (int)((k + 1) * least + min(k + 1, more));
+            const float size = (float)r.cnt * __builtin_amdgcn_rcpf((float)len);
+            const auto begin = [&](int k) { return k == len ? r.cnt : min((int)__builtin_fmaf((float)k, size, 0.0625f), r.cnt); }; // (a whole number may have come out a little less)
+            to = begin(from + 1), from = begin(from);
         } else {
             to = min(r.cnt, from + (int)(end - x));
             w0 = sh.owner(x - (uint32_t)from), w1 = sh.owner(x - (uint32_t)from + (uint32_t)r.cnt - 1);
@@ -512,7 +517,7 @@ template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_b
                 o[0] = float4_t{u0[0], u1[0], u0[1], u1[1]}, o[1] = float4_t{u0[2], u1[2], u0[3], u1[3]};
             }
         }
-        __syncthreads();
+        meet();
         constexpr int PER_ROW = W * 64 / (16 * QT); // threads
         const int row = (int)threadIdx.x / PER_ROW, mr = m0 + row;
         if (mr < M) {
@@ -541,7 +546,7 @@ template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_b
                 } else *(float4_t *)(a.part + left * D + at4 * 4) = o;
             }
         }
-        __syncthreads();
+        meet();
         x += per > 0 ? 1 : (uint32_t)(to - from);
     }
 }

@@ -24,7 +24,7 @@ typedef struct {
     uint16_t *out;
     float *part, *ml; /* partial results: [2 grid][16 QT][dim], and of each row its maximum and its sum */
     void *parts;      /* [2 grid] */
-    qwk_div by_group;
+    qwk_div by_group, by_grid;
     uint32_t q_stride, out_stride, group, window, grid;
     float scale; /* of a score, log2(e) in it */
 } qwk_attn_args;
