@@ -660,8 +660,8 @@ __device__ __forceinline__ uint32_t quantise(uint32_t x, uint16_t &scale) {
 }
 
 // `waves` waves of a row take its heads in turn, queries, then keys, then values, two values a lane (four where a head has more than 128). Sines and cosines of the positions, in 64
-// bits, are made once a wave. Four tokens of values lie beside one another in the cache: the wave of the first one's row stores all of them that are rows of this step. Sixteen rows
-// in a row go to one XCD, whose cache then holds whole lines of their units.
+// bits, are made once a wave. Four tokens of values lie beside one another in the cache: the waves of those of them that are rows of this step share the heads, a wave storing all four
+// tokens of its own (the first row's waves alone took 6 of 42 us longer over 4096 rows). Sixteen rows in a row go to one XCD, whose cache then holds whole lines of their units.
 template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(const qwk_kv_write_args &a) {
     constexpr uint32_t N = 4, W = QW_WG_KV / 64; // heads in hand at once
     const qwk_kv &c = a.c;
@@ -748,9 +748,21 @@ template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(co
             for (uint32_t k = 0; k < C; k++) {
                 if (2 * d[k] >= D) continue;
                 uint32_t r = x[n][k];
-                if (2 * d[k] < a.rot) // (an even number: both values turn or neither)
-                    r = half_bits((double)half_of((uint16_t)r) * cs[k][0] + (double)half_of((uint16_t)y[n][k]) * sn[k][0]) |
-                        (uint32_t)half_bits((double)half_of((uint16_t)(r >> 16)) * cs[k][1] + (double)half_of((uint16_t)(y[n][k] >> 16)) * sn[k][1]) << 16;
+                if (2 * d[k] < a.rot) { // (an even number: both values turn or neither)
+                    // In 32 bits with a bound on what that is off by: the factors and one product half a step of 24 bits each, the sum half a step of its own. Where both ends of the interval
+                    // round to the same half, that is the result; the others, one value in a thousand or so (and zeros, whose sign the bound does not tell), are made in 64 bits.
+                    uint32_t lo = 0, hi = 0;
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; e++) {
+                        const float u = half_of((uint16_t)(r >> 16 * e)), w = half_of((uint16_t)(y[n][k] >> 16 * e)), uc = u * (float)cs[k][e], ws = w * (float)sn[k][e];
+                        const float sum = __builtin_fmaf(w, (float)sn[k][e], uc), off = __builtin_fmaf(__builtin_fabsf(uc) + __builtin_fabsf(ws), 0x3.1p-24f, 0x1p-120f);
+                        lo |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(sum - off)) << 16 * e, hi |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(sum + off)) << 16 * e;
+                    }
+                    if (__builtin_expect(lo != hi, 0))
+                        lo = half_bits((double)half_of((uint16_t)r) * cs[k][0] + (double)half_of((uint16_t)y[n][k]) * sn[k][0]) |
+                             (uint32_t)half_bits((double)half_of((uint16_t)(r >> 16)) * cs[k][1] + (double)half_of((uint16_t)(y[n][k] >> 16)) * sn[k][1]) << 16;
+                    r = lo;
+                }
                 if (h < a.q_heads) ((uint32_t *)(a.q_out + (size_t)row * a.qo_stride + (size_t)h * D))[d[k]] = r;
                 else if (TYPE == F16) {
                     if (unit) *(uint32_t *)(unit + place<F16>(D, false, t, 2 * d[k])) = r;
@@ -763,20 +775,20 @@ template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(co
             }
         }
     }
-    if (!unit0 || (t % 4 && (int)row != s.first)) return;
-    const uint32_t rows = min(4 - t % 4, (uint32_t)(s.first + s.n) - row);
-    for (uint32_t h = (mine < qk ? mine + (qk - mine + step - 1) / step * step : mine); h < qk + c.heads; h += step) {
-        uint8_t *const unit = unit0 + (h - qk) * head_bytes(c);
+    if (!unit0) return;
+    const uint32_t before = min(t % 4, row - (uint32_t)s.first), row0 = row - before, t0 = t - before, rows = min(4 - t0 % 4, (uint32_t)(s.first + s.n) - row0); // the rows of the four tokens
+    for (uint32_t h = (before + 1) * step - 1 - mine; h < c.heads; h += rows * step) {
+        uint8_t *const unit = unit0 + h * head_bytes(c);
         uint32_t x[4][C];
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++)
 #pragma unroll
-            for (uint32_t k = 0; k < C; k++) x[j][k] = j < rows && 2 * d[k] < D ? ((const uint32_t *)(a.v + (size_t)(row + j) * a.v_stride + (size_t)(h - qk) * D))[d[k]] : 0;
+            for (uint32_t k = 0; k < C; k++) x[j][k] = j < rows && 2 * d[k] < D ? ((const uint32_t *)(a.v + (size_t)(row0 + j) * a.v_stride + (size_t)h * D))[d[k]] : 0;
 #pragma unroll
         for (uint32_t k = 0; k < C; k++) {
             if (2 * d[k] >= D) continue;
             if (TYPE == F16) {
-                uint16_t *to = (uint16_t *)(unit + place<F16>(D, true, t, 2 * d[k])); // the second value four tokens on
+                uint16_t *to = (uint16_t *)(unit + place<F16>(D, true, t0, 2 * d[k])); // the second value four tokens on
                 if (rows == 4)
                     *(uint4_t *)to = uint4_t{(x[0][k] & 0xffff) | x[1][k] << 16, (x[2][k] & 0xffff) | x[3][k] << 16, x[0][k] >> 16 | (x[1][k] & 0xffff0000u), x[2][k] >> 16 | (x[3][k] & 0xffff0000u)};
                 else
@@ -788,7 +800,7 @@ template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(co
                 uint16_t scale[4];
 #pragma unroll
                 for (uint32_t j = 0; j < 4; j++) q[j] = quantise(x[j][k], scale[j]);
-                uint8_t *to = unit + place<Q8>(D, true, t, 2 * d[k]), *scales = unit + place_scale(D, true, t, 2 * d[k]);
+                uint8_t *to = unit + place<Q8>(D, true, t0, 2 * d[k]), *scales = unit + place_scale(D, true, t0, 2 * d[k]);
                 if (rows == 4) {
                     *(uint2_t *)to = uint2_t{(q[0] & 0xff) | (q[1] & 0xff) << 8 | (q[2] & 0xff) << 16 | q[3] << 24, q[0] >> 8 | (q[1] & 0xff00) | (q[2] & 0xff00) << 8 | (q[3] & 0xff00) << 16};
                     if (lane % 16 == 0) *(uint2_t *)scales = uint2_t{scale[0] | (uint32_t)scale[1] << 16, scale[2] | (uint32_t)scale[3] << 16};
