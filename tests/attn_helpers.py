@@ -132,8 +132,6 @@ def attention(cache, step, query, scale, window=0, dead=()):
         if not seen:
             continue
         k, v = cache.get(step.table, slot, seen)
-        with np.errstate(over="ignore"):
-            v = v.astype(np.float16).astype(np.float64)  # as they are read back
         qr = query[row].astype(np.float64).reshape(cache.heads, G, D)
         s = np.einsum("hgd,thd->hgt", qr, k) * scale
         size = (np.einsum("hgd,thd->hgt", np.abs(qr), np.abs(k)) * scale).max(-1, keepdims=True)
@@ -149,7 +147,7 @@ def tolerance(o, weight, size, T, D):
     """The result is rounded to binary16 once: half a step, 2^-11 of it, or 2^-25 where binary16 steps are 2^-24. A score is a sum of D products in binary32 (2^-24 a step, D steps at
     most, of at most `size` = scale * sum |q k|), times a scale rounded to 24 bits and log2(e) (two more steps), brought to its weight by a subtraction and an exponential
     (another two steps of the score's size, 2^-22 for the exponential): relative error e of a weight, which enters numerator and denominator. The weights of the second product
-    are held in 21 bits; its sums over T tokens run in tiles of 16, each lane's over T / 4 of them at most: T / 4 + 8 steps of 2^-24 of sum p |v|, as do those of the
+    are held in 21 bits, and the product of their last ten with a value's last seven, 2^-21 of the whole at most, is left out; its sums over T tokens run in tiles of 16, each lane's over T / 4 of them at most: T / 4 + 8 steps of 2^-24 of sum p |v|, as do those of the
     denominator. `weight` = sum p |v|. (The caller adds what the smallest weights lose: half of binary16's last step, 2^-25, where the largest weight is 2^14, each times a value.)"""
     e = (D + 6) * 2.0 ** -24 * size + 2.0 ** -22
-    return 2.0 ** -11 * np.abs(o.reshape(weight.shape)) + 2.0 ** -25 + weight * (2 * e + 2.0 ** -21 + 2 * (T / 4 + 8) * 2.0 ** -24)
+    return 2.0 ** -11 * np.abs(o.reshape(weight.shape)) + 2.0 ** -25 + weight * (2 * e + 2.0 ** -20 + 2 * (T / 4 + 8) * 2.0 ** -24)
