@@ -56,7 +56,7 @@ typedef struct {
     uint32_t vocab, stride, tiles;
 } qwk_sample_args;
 #define QW_WG_SAMPLE 1024u
-#define QW_WG_SAMPLE_BINS 512u
+#define QW_WG_SAMPLE_BINS 1024u
 #define QW_SAMPLE_TILE 8192u      /* tokens of a workgroup of the first launch */
 #define QW_SAMPLE_BINS 256u
 #define QW_SAMPLE_STARTS 264u     /* QW_SAMPLE_BINS + 1, and to a multiple of eight */

@@ -189,7 +189,7 @@ __device__ __forceinline__ void sample_row(SampleShared &s, const qwk_sample_arg
 // the tiles' bins up; then a filter's border lies in a bin whose tokens are known, some thousand of them at most as a rule: 256 finer bins, then each of the few in one of these
 // against all others. The token drawn is found by the tiles' sums and one tile. A border in the last bin (what lies 31 below the largest), or in a bin or finer bin of too many
 // tokens, goes the slow way (sample_row).
-constexpr uint32_t REST = QW_SAMPLE_BINS - 1, LIST = 8192, FEW = 1024, NEAR = 1024, NEAR_TILES = 32, TILES = QW_SAMPLE_VOCAB / QW_SAMPLE_TILE;
+constexpr uint32_t REST = QW_SAMPLE_BINS - 1, LIST = 8192, FEW = 1024, SMALL = 256, NEAR = 1024, NEAR_TILES = 32, TILES = QW_SAMPLE_VOCAB / QW_SAMPLE_TILE;
 __device__ __forceinline__ int grid_of(float l) { return (int)fminf(fmaxf(floorf(l * 8.f), -1e9f), 1e9f); }
 __device__ __forceinline__ uint32_t finer(float l, int g) { return 255u - (uint32_t)fminf(fmaxf((l * 8.f - (float)g) * 256.f, 0.f), 255.f); } // within a bin, from its top down
 
@@ -358,9 +358,9 @@ struct FastSampler {
         return true;
     }
     // The border of a filter: the last token kept, of those that `want` tokens (or weight) reach. Leaves it in cut_key and cut_id, and what it and those before it weigh in all.
-    __device__ bool border(bool weights, u64 want) {
+    __device__ bool border(bool weights, u64 want, bool found) { // found: the bin is known (pick)
         const uint32_t t = threadIdx.x;
-        find<QW_SAMPLE_BINS>(s.weight, s.count, weights, want);
+        if (!found) find<QW_SAMPLE_BINS>(s.weight, s.count, weights, want);
         const int bin = (int)s.pick;
         const u64 bn = s.before_n, bw = s.before_w;
         if (bin == (int)REST || !load(bin)) return false;
@@ -416,6 +416,58 @@ struct FastSampler {
         return true;
     }
 };
+
+// A row whose first filter leaves some hundred tokens at most, all of them at hand: the filters and the draw by comparing each with all others, in descending order and then by number.
+__device__ __forceinline__ void sample_few(SampleFast &s, const qwk_sample_args &a, uint32_t row, const qwk_sample_row &p, const Weigh &weigh, float top, u64 all) {
+    const uint32_t t = threadIdx.x, n = s.few, each = n <= 64 ? 64 : SMALL, j = t % each, parts = QW_WG_SAMPLE / each;
+    const bool mine = j < n;
+    const uint32_t key = mine ? s.few_key[j] : 0, id = mine ? s.few_id[j] : 0;
+    const u64 own = mine ? s.few_weight[j] : 0;
+    u64 w = 0;
+    uint32_t c = 0;
+    if (t < each) s.fine_weight[t] = 0, s.fine_count[t] = 0;
+    if (t == 0) s.all = all, s.below = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = t / each; i < n; i += parts) {
+        const uint32_t k = s.few_key[i], d = s.few_id[i];
+        const u64 x = s.few_weight[i];
+        const bool before = k > key || (k == key && d < id);
+        c += before, w += before ? x : 0;
+    }
+    if (c) atomicAdd(&s.fine_count[j], c), atomicAdd(&s.fine_weight[j], w);
+    __syncthreads();
+    const bool by_count = p.top_k && p.top_k < a.vocab;
+    const uint32_t keep = by_count ? min(p.top_k, n) : n;
+    c = s.fine_count[j], w = s.fine_weight[j];
+    if (by_count && t < n && c == keep - 1) s.all = w + own; // of what top-k leaves
+    __syncthreads();
+    bool kept = mine && c < keep;
+    if (p.top_p < 1) {
+        u64 want = (u64)ceil((double)fmaxf(p.top_p, 1e-30f) * (double)s.all);
+        want = want < 1 ? 1 : want > s.all ? s.all : want;
+        kept = kept && w < want;
+    }
+    if (p.min_p > 0) kept = kept && own >= (u64)((double)fminf(p.min_p, 1.f) * (double)weigh(top));
+    if (t < each) s.few_weight[t] = kept ? own : 0, s.fine_weight[t] = 0;
+    __syncthreads();
+    u64 below = 0, some = 0;
+#pragma unroll 4
+    for (uint32_t i = t / each; i < n; i += parts) {
+        const u64 x = s.few_weight[i];
+        some += x, below += s.few_id[i] < id ? x : 0;
+    }
+    if (below && mine) atomicAdd(&s.fine_weight[j], below);
+    if (j == 0 && some) atomicAdd(&s.below, some);
+    __syncthreads();
+    const u64 whole = s.below, from = s.fine_weight[j], x = s.few_weight[j];
+    const double u = (double)a.u[row];
+    const u64 at = u > 0 ? min((u64)(u * (double)whole), whole - 1) : 0; // the first token whose sum with those before it is larger
+    if (t < n && from <= at && at < from + x) {
+        a.ids[row] = id;
+        if (a.probs) a.probs[row] = (float)((double)x / (double)whole);
+    }
+}
 
 // false: the slow way has to be taken
 __device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t row) {
@@ -502,11 +554,33 @@ __device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t ro
         for (uint32_t i = lane; i < QW_SAMPLE_BINS; i += 64) all += s.weight[i];
         all = of_lane(wave_up(all), 63);
     }
+    const auto share = [&] { want = (u64)ceil((double)fmaxf(p.top_p, 1e-30f) * (double)all), want = want < 1 ? 1 : want > all ? all : want; };
+    if (by_count || by_weight) {
+        if (!by_count) share();
+        f.find<QW_SAMPLE_BINS>(s.weight, s.count, !by_count, want);
+        const uint32_t last = s.pick;
+        if (near && last != REST && s.before_n + s.count[last] <= SMALL) { // every token down to that bin, if the tokens at hand are all of them
+            if (t == 0) s.few = 0, s.slow = 0;
+            __syncthreads();
+            const uint32_t tile = t / near, i = t % near;
+            if (tile < a.tiles && s.off[tile] <= (int)last) {
+                const uint32_t end = s.starts[tile * (QW_SAMPLE_BINS + 1) + (last - (uint32_t)s.off[tile]) + 1];
+                if (end > near) s.slow = 1;
+                else if (i < end) {
+                    const uint32_t k = atomicAdd(&s.few, 1u);
+                    s.few_key[k] = near_key, s.few_id[k] = near_id, s.few_weight[k] = weigh(of_key(near_key));
+                }
+            }
+            __syncthreads();
+            if (!s.slow) return sample_few(s, a, row, p, weigh, top, all), true;
+        }
+    }
+    bool found = true;
 #pragma unroll 1
-    for (int pass = by_count ? 0 : 1; pass < (by_weight ? 2 : 1); pass++) { // (one after the other through the same code)
-        if (pass) want = (u64)ceil((double)fmaxf(p.top_p, 1e-30f) * (double)all), want = want < 1 ? 1 : want > all ? all : want;
+    for (int pass = by_count ? 0 : 1; pass < (by_weight ? 2 : 1); pass++, found = false) { // (one after the other through the same code)
+        if (pass) share();
         __syncthreads();
-        if (!f.border(pass, want)) return false;
+        if (!f.border(pass, want, found)) return false;
         all = s.all;
         if (s.cut_key > cut_key || (s.cut_key == cut_key && s.cut_id < cut_id)) cut_key = s.cut_key, cut_id = s.cut_id, edge = g - grid_of(of_key(cut_key));
     }

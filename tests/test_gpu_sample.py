@@ -150,3 +150,17 @@ def test_extreme_settings(gpu):
 def test_without_probabilities(gpu):
     rng = np.random.default_rng(6)
     check(gpu, model_like(rng, 3, 777), np.array(SETTINGS[:3], ROW), rng.random(3, dtype=np.float32), probs=False)
+
+
+@pytest.mark.parametrize("V,first,spread", [(20000, 100, 20000), (20000, 100, 100), (131072, 250, 131072), (8192, 64, 8192), (300, 30, 300), (131072, 40, 20000)])
+def test_few_tokens_left(gpu, V, first, spread):
+    """Some tens or hundreds of tokens far above all others, over the whole row or side by side (more in one stretch of it than are at hand), many of them equal; a filter's border among them."""
+    rng = np.random.default_rng(V + first + spread)
+    B = 24
+    logits = rng.standard_normal((B, V)).astype(np.float32)
+    for b in range(B):
+        at = rng.permutation(spread)[:first]
+        logits[b, at] = 9 + (rng.integers(0, 12, first) / 4 if b % 2 else rng.standard_normal(first))
+    k = rng.integers(2, first, B)
+    params = np.array([(0.8, *((0.9, 0.0), (1.0, 0.0), (0.95, 0.05), (1.0, 0.3))[b % 4], k[b] if b % 3 else 0) for b in range(B)], ROW)
+    check(gpu, logits, params, rng.random(B).astype(np.float32))
