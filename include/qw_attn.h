@@ -94,7 +94,8 @@ bool qw_sample(qw_batch *b, int rows, int vocab, int stride, const qw_at *logits
 /* A recorder for callers with streams and memory of their own (a framework's tensors, a stream under graph capture): begin, any of the
  * functions above, end. The launches go to `stream` (a hipStream_t of this device; NULL: the default stream), in order, and end returns without
  * waiting; nothing is allocated, copied or synchronised. Buffers have to be device-only: qw_hip_buf_new_device, or views. It holds
- * 64 launches (qw_attn and qw_sample make two each); a call that finds no room fails. One recorder at a time per device (NULL + qw_hip_last_error otherwise); qw_hip_stream_end gives it back and launches nothing where a function failed.
+ * 64 launches (qw_attn and qw_sample make two each); a call that finds no room fails. One recorder at a time per device (NULL + qw_hip_last_error
+ * otherwise); qw_hip_stream_end gives it back and launches nothing where a function failed.
  * qw_path_gg_moe_noalloc uses the same one. */
 qw_batch *qw_hip_stream_begin(qw_gpu *g, void *stream);
 bool qw_hip_stream_end(qw_batch *b);

@@ -21,11 +21,19 @@ enum { F16 = 1, Q8 = 8 };
 // through LDS between the two; the cache's units are stored so that a lane's operands are 16 consecutive bytes of a wave's 1024.
 //
 // Work: a pair is (slot, head, block of 16 QT of the slot's rows x query heads of that head), with its tiles of 32 tokens. As a rule a pair is cut into as many equal shares as it has
-// times `size` tiles, a workgroup each, with the least `size` (of whole rounds of the four waves) that the grid has workgroups for: nobody then begins twice. Where pairs are many and
+// times `size` tiles, a workgroup each, with the least `size` that the grid, a workgroup a compute unit, has workgroups for: nobody then begins twice. Where pairs are many and
 // unlike, that would leave some workgroups with much more than others; their tiles then lie one behind another, pair after pair, and the workgroups take equal shares of that line,
-// wherever pairs begin or end in it (Shares). All of it follows from first[] and len[] on the device, so a captured call goes on being right, and even, as the slots grow. What a
-// share makes of a pair that others have shares of it leaves as (maximum, sum, unnormalised result), and qwk_attn_join puts these together in the order of the shares: the same
-// bits every time.
+// wherever pairs begin or end in it (Shares). (Lines for everything: 16 chats 22.7 us instead of 20.9, 12 slots of drafts 34.5 instead of 30.0.) All of it follows from first[] and len[]
+// on the device, so a captured call goes on being right, and even, as the slots grow. What a share makes of a pair that others have shares of it leaves as (maximum, sum, unnormalised
+// result), and qwk_attn_join puts these together in the order of the shares: the same bits every time.
+//
+// Eight waves a workgroup take a share's tiles in turn, each with the next step's units on their way while it works on the last; two workgroups of four a compute unit left twice as much for
+// the join (drafts 32.3 us, not 29.4; one token over 700 tokens 11.9, not 12.1). A wave with two blocks of queries of 192 or 256 values needs all of a SIMD's registers: four waves there.
+//
+// Bound: by the cache's bytes once there are enough of them. 64 slots of 8192 tokens, binary16, 4 heads of 128 values (1.07 GB) 178 us, 5.9 TB/s; one slot of 131072, Q8_0, 2 heads of 256
+// (143 MB) 30 us and 5 for the join; 16 slots of up to 4096, binary16 (78 MB) 17 and 4. Two blocks of queries make Q8_0 instruction-bound (a step, two units of 128 values, is some
+// 500 vector and 64 matrix instructions): 12 slots of 45 rows over 6001 tokens 23 us for 55 MB, of which 4 are gone before the first unit arrives. One token over 700: 8.4 us, five
+// dependent round trips to memory and the launch.
 
 struct Slot { int n, len, first; }; // rows, tokens, first row
 
@@ -556,7 +564,8 @@ template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_b
 }
 
 // Results of pairs that several workgroups share, put together by as many: of the pair's results, workgroup w takes its part, and its threads share
-// what the others left of them. A pair of 256 shares (8 rows of 256 values, 131072 tokens) costs a thread two loads, as one of two shares does.
+// what the others left of them. A pair of 128 shares (8 rows of 256 values, 131072 tokens) costs a thread a load or two, as one of two shares does. 4 to 6 us: two round trips and the launch
+// (one workgroup a pair took 28 for that one). A launch of its own, because the workgroup that comes last would have to be told apart by a counter, and the workspace need not be cleared.
 template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args &a) {
     __shared__ float4_t so[QW_WG_JOIN];
     __shared__ float sm[QW_WG_JOIN], sl[QW_WG_JOIN];
@@ -666,6 +675,8 @@ __device__ __forceinline__ uint32_t quantise(uint32_t x, uint16_t &scale) {
 // `waves` waves of a row take its heads in turn, queries, then keys, then values, two values a lane (four where a head has more than 128). Sines and cosines of the positions, in 64
 // bits, are made once a wave. Four tokens of values lie beside one another in the cache: the waves of those of them that are rows of this step share the heads, a wave storing all four
 // tokens of its own (the first row's waves alone took 6 of 42 us longer over 4096 rows). Sixteen rows in a row go to one XCD, whose cache then holds whole lines of their units.
+// 4096 rows of 32 + 4 heads of 128 values, Q8_0: 29 us, 80 MB at 2.7 TB/s (of them the values 5, turning 4, queries out 4, positions 2: the rest is rows in and the chain
+// of slot, positions, angles in front of them). A row: 3.8 us, that chain.
 template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(const qwk_kv_write_args &a) {
     constexpr uint32_t N = 4, W = QW_WG_KV / 64; // heads in hand at once
     const qwk_kv &c = a.c;
@@ -824,7 +835,8 @@ extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f1_c2(qwk_kv
 extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f8_c1(qwk_kv_write_args a) { kv_write_body<Q8, 1>(a); }
 extern "C" __global__ __launch_bounds__(QW_WG_KV) void qwk_kv_write_f8_c2(qwk_kv_write_args a) { kv_write_body<Q8, 2>(a); }
 
-// A wave a unit of a slot's rows, a head, and keys or values: it takes the unit as it lies, 16 bytes a lane, and deals it out to the rows. Bound by the rows out.
+// A wave a unit of a slot's rows, a head, and keys or values: it takes the unit as it lies, 16 bytes a lane, and deals it out to the rows. Bound by the rows out: 16384 rows of 4 heads of
+// 128 values out of Q8_0 10.5 us, 51 MB at 4.9 TB/s; 333 rows 7.2, slots, page, unit, rows out one behind the other.
 template <int TYPE> __device__ __forceinline__ void kv_read_body(const qwk_kv_read_args &a) {
     const qwk_kv &c = a.c;
     const uint32_t lane = threadIdx.x & 63, D = c.dim, task = __builtin_amdgcn_readfirstlane(blockIdx.x * (QW_WG_KV / 64) + (threadIdx.x >> 6));
