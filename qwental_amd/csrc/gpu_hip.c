@@ -2563,8 +2563,8 @@ static bool tr_attn(qw_batch *b) {
     qw_span in[QW_KV_READS], q, out;
     if (!kv_bind(b, &x, &a.c, false, &in)) return false;
     if (x.q_heads < 1 || x.q_heads > QW_ATTN_MAX_Q_HEADS || x.q_heads % x.heads) return fail(b, "attn_paged: %d query heads for %d of keys (a multiple, up to %d)", x.q_heads, x.heads, QW_ATTN_MAX_Q_HEADS);
-    // tiles of all pairs are counted in 32 bits
-    if ((((uint64_t)x.rows * (uint64_t)x.q_heads + 15) / 16 + (uint64_t)x.slots * (uint64_t)x.heads) * ((uint64_t)x.max_pages * (uint64_t)x.page / QW_ATTN_TILE + 2) > INT32_MAX)
+    // tiles of all pairs are counted in 31 bits, the grid's size behind them
+    if ((((uint64_t)x.rows * (uint64_t)x.q_heads + 15) / 16 + (uint64_t)x.slots * (uint64_t)x.heads) * ((uint64_t)x.max_pages * (uint64_t)x.page / QW_ATTN_TILE + 2) > 1 << 30)
         return fail(b, "attn_paged: %d rows of %d query heads over up to %lld tokens: too many for one call", x.rows, x.q_heads, (long long)x.max_pages * x.page);
     if (x.window < 0 || !(x.scale >= 0) || x.scale > 1e30f) return fail(b, "attn_paged: window %d, scale %g", x.window, (double)x.scale);
     if (!kv_rows(b, 4, false, &x, x.q_heads, x.stride[0], "q", (uint16_t **)&a.q, &a.q_stride, &q) || !kv_rows(b, 5, true, &x, x.q_heads, x.stride[1], "out", &a.out, &a.out_stride, &out)) return false;
@@ -2630,6 +2630,7 @@ void qw_batch_dispatch(qw_batch *b, unsigned gx, unsigned gy, unsigned gz, unsig
     (void)gz; (void)tx; (void)ty; (void)tz;
     if (b->failed) return;
     if (!b->k) { fail(b, "qw_batch_dispatch without a kernel"); return; }
+    if (b->own_stream && !of_attn_family(b->k->fam)) { fail(b, "%s: a recorder on a stream takes the functions of qw_attn.h", b->k->name); return; }
     b->allow_released = false;
     const int first = b->nl;
     bool ok;
@@ -3161,13 +3162,13 @@ static bool submit_segment(qw_batch *b, bool last) {
 }
 
 void qw_batch_flush(qw_batch *b) {
-    if (b->prof) return; // as in the reference: a profiled batch is not split
+    if (b->prof || b->own_stream) return; // as in the reference: a profiled batch is not split
     if (b->nseg >= 8) return;
     submit_segment(b, false);
 }
 
 void qw_batch_submit(qw_batch *b) {
-    if (b->submitted) return;
+    if (b->submitted || b->own_stream) return;
     b->submitted = true;
     submit_segment(b, false);
 }
@@ -3298,6 +3299,12 @@ double qw_hip_batch_end_parts(qw_batch *b, double *secs) {
     return qw_batch_end(b);
 }
 double qw_batch_end(qw_batch *b) {
+    if (b->own_stream) { // not a batch: nothing of it is launched
+        b->failed = true;
+        (void)qw_hip_stream_end(b);
+        set_err(b->g, "qw_batch_end: a recorder on a stream ends with qw_hip_stream_end");
+        return -1;
+    }
     if (b->submitted) return batch_wait(b, false);
     b->submitted = true;
     submit_segment(b, true);

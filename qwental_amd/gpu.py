@@ -281,7 +281,8 @@ class Batch:
 
 
 class StreamBatch(Batch):
-    """A recorder on a stream of the caller's (include/qw_attn.h): end() launches and returns without waiting."""
+    """A recorder on a stream of the caller's (include/qw_attn.h): end() launches and returns without waiting, drop() gives it back and launches nothing. Used in a
+    with statement it ends at the block's end, or is dropped where the block raises."""
 
     def __init__(self, gpu, stream=None):
         self.gpu, self.L = gpu, gpu.L
@@ -293,6 +294,25 @@ class StreamBatch(Batch):
         b, self.b = self.b, None
         if not self.L.qw_hip_stream_end(b):
             raise RuntimeError("GPU launches failed: " + self.gpu.last_error())
+
+    def drop(self):
+        b, self.b = self.b, None
+        if b and self.gpu.g:
+            self.L.qw_batch_kernel(b, None)
+            self.L.qw_batch_dispatch(b, 1, 1, 1, 1, 1, 1)  # without a kernel: the recorder has failed
+            self.L.qw_hip_stream_end(b)
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, kind, value, trace):
+        if kind is None:
+            self.end()
+        else:
+            self.drop()
+
+    def __del__(self):
+        self.drop()
 
 
 class View(Buf):

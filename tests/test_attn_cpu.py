@@ -323,6 +323,17 @@ int main(void) {
     for (int i = 0; i < 64; i++)
         if (!call(b, READ, &a)) return printf("launch %d: %s\n", i, g->err), 1;
     if (call(b, READ, &a) || !strstr(qw_hip_last_error(g), "64 launches") || qw_hip_stream_end(b) || launches != before) return printf("65 launches\n"), 1;
+    // not a batch: it is neither split nor ended as one, and takes no other functions
+    b = qw_hip_stream_begin(g, NULL);
+    qw_batch_flush(b), qw_batch_submit(b);
+    if (!b || !call(b, READ, &a) || qw_batch_end(b) >= 0 || !strstr(qw_hip_last_error(g), "qw_hip_stream_end") || launches != before) return printf("ended as a batch\n"), 1;
+    qw_path *op = qw_path_open(g, 1024, 256, 64, 4, 16, true);
+    qw_buf ow;
+    if (!qw_hip_buf_new_device(g, (size_t)64 * 1024 * 256 * 2, &ow)) return 3;
+    b = qw_hip_stream_begin(g, NULL);
+    const qw_tensor OW = {.buf = &ow, .type = 8};
+    if (!b || (qw_path_qmv_gg(op, b, &OW, 64, 256, &B[4], 0, &B[5], 0, 1, true) && qw_hip_stream_end(b)) || !strstr(qw_hip_last_error(g), "qw_attn.h") || launches != before) return printf("another function: %s\n", g->err), 1;
+    if (g->na_busy) (void)qw_hip_stream_end(b);
     // other devices' streams, and the current device put back
     if (qw_hip_stream_begin(g, (void *)0x2000) || qw_hip_stream_begin(g, (void *)0x3000) || qw_hip_stream_begin(NULL, NULL) || qw_hip_stream_end(NULL)) return printf("streams\n"), 1;
     current_device = 3;

@@ -220,10 +220,9 @@ class Torch:
         self.ids.fill_(-7)
 
     def run(self, stream):
-        b = self.gpu.stream(stream)
-        for c in self.calls:
-            c(b)
-        b.end()
+        with self.gpu.stream(stream) as b:
+            for c in self.calls:
+                c(b)
 
     def verify(self):
         freq, qh, kh = self.freq.cpu().numpy(), self.q.cpu().numpy(), self.k.cpu().numpy()
@@ -306,6 +305,11 @@ def test_recorder_is_given_back(gpu, dev):
     with pytest.raises(RuntimeError):
         b.end()
     host.free()
+    with pytest.raises(ZeroDivisionError):
+        with gpu.stream(stream) as b:
+            t.calls[0](b)
+            1 // 0
+    gpu.stream(stream)  # (nobody holds it)
     t.run(stream)
     t.verify()
     with pytest.raises(RuntimeError, match="not memory"):
