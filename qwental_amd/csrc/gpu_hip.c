@@ -229,8 +229,7 @@ static const qw_wg_rule wg_rules[] = {
     {"qwk_moe_prep", QW_WG_PREP, 0, 0},
     {"qwk_hc_up", QW_WG_HC_UP, 0, 0},
     {"qwk_attn_join", QW_WG_JOIN, 0, 0},
-    {"qwk_attn_w8_", 512, 0, 0},
-    {"qwk_attn_w4_", 256, 0, 0},
+    {"qwk_attn_", QW_WG_ATTN, 0, 0},
     {"qwk_kv_", QW_WG_KV, 0, 0},
     {"qwk_sample_bins", QW_WG_SAMPLE_BINS, 0, 0},
     {"qwk_sample", QW_WG_SAMPLE, 0, 0},
@@ -2528,11 +2527,15 @@ static bool tr_kv_write(qw_batch *b) {
     static const char *const reads[] = {"k", "v", "freq", "pos", "q"};
     if (!apart_all(b, &qo, "q_out", 4, read, reads) || !apart_all(b, &qo, "q_out", QW_KV_READS, in, kv_reads) || !apart_all(b, &in[0], "the cache", 5, read, reads)) return false;
     a.q_heads = (uint32_t)x.q_heads, a.rot = (uint32_t)x.rot, a.axes = (uint32_t)x.axes, a.pairs0 = (uint32_t)x.pairs[0], a.pairs1 = (uint32_t)x.pairs[1], a.adjacent = x.adjacent != 0;
-    // A wave a head while that makes no more than eight waves for each SIMD of the device, then several heads a wave: what a row costs before its first head is then shared
-    const unsigned heads = (unsigned)(x.q_heads + 2 * x.heads), waves = (unsigned)b->g->ncu * 32 / (unsigned)x.rows;
-    a.waves = waves < 1 ? 1 : umin(waves, heads);
+    // Waves of a row: one a head while there are few rows; then a wave takes four heads at a time, and as many times four as leave the device eight waves a SIMD at most, which share what a row costs
+    // before its first head. 32 + 4 + 4 heads of 128 values, Q8_0, with the rows' reading back: 64 rows 8.1 us with a wave a head, 9.8 with nine waves; 256 rows 12.5 and 11.3; 1024 rows 16.6 with five
+    // and 18.8 with nine; 4096 rows 34.3 with two, 37.1 with five and 36.2 with one.
+    const unsigned R = (unsigned)x.rows, qk = (unsigned)(x.q_heads + x.heads), ncu = (unsigned)b->g->ncu;
+    a.waves = qk + (unsigned)x.heads;
+    if (R * a.waves > 20 * ncu)
+        for (unsigned r = 1; (a.waves = cdiv(qk, 4 * r)) > 1 && R * a.waves > 32 * ncu;) r++;
     static const char *const names[2][2] = {{"qwk_kv_write_f1_c1", "qwk_kv_write_f1_c2"}, {"qwk_kv_write_f8_c1", "qwk_kv_write_f8_c2"}};
-    return add_launch(b, names[x.type == 8][x.dim > 128], cdiv((unsigned)x.rows * a.waves, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
+    return add_launch(b, names[x.type == 8][x.dim > 128], cdiv(R * a.waves, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
 }
 static bool tr_kv_read(qw_batch *b) {
     qw_attn_geo x;
@@ -2545,10 +2548,10 @@ static bool tr_kv_read(qw_batch *b) {
     const unsigned units = (unsigned)x.rows / QW_UNIT + 2 * umin((unsigned)x.slots, (unsigned)x.rows);
     return add_launch(b, x.type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", cdiv(units * 2 * (unsigned)x.heads, QW_WG_KV / 64), QW_WG_KV, &a, sizeof a);
 }
-// A workgroup a compute unit: eight waves, or four where a wave has all of a SIMD's registers; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
+// A workgroup a compute unit; what they leave for the join: results and, of each row, maximum and sum, at the largest block of rows.
 static unsigned attn_grid(const qw_gpu *g) { return (unsigned)g->ncu; }
-static size_t attn_part_bytes(const qw_gpu *g, int dim, unsigned qt) { return (size_t)attn_grid(g) * 2 * 16 * qt * (size_t)dim * 4; }
-size_t qw_attn_ws_bytes(const qw_gpu *g, int dim) { return !g || dim < 64 || dim > 256 || dim % 64 ? 0 : attn_part_bytes(g, dim, 2) + attn_part_bytes(g, 2, 2) + (size_t)attn_grid(g) * 2 * QW_ATTN_PART; }
+static size_t attn_rows(const qw_gpu *g, int dim) { return (size_t)attn_grid(g) * 2 * (dim <= 128 ? 32 : 16); }
+size_t qw_attn_ws_bytes(const qw_gpu *g, int dim) { return !g || dim < 64 || dim > 256 || dim % 64 ? 0 : attn_rows(g, dim) * ((size_t)dim + 2) * 4 + (size_t)attn_grid(g) * 2 * QW_ATTN_PART; }
 // Division by d for dividends below 2^31: with 2^l >= d the least such power, mul = floor(2^(31 + l) / d) + 1 is off by less than 2^l / 2^31 of a step for each of them.
 static qwk_div div_of(uint32_t d) {
     unsigned l = 0;
@@ -2556,8 +2559,8 @@ static qwk_div div_of(uint32_t d) {
     return d <= 1 ? (qwk_div){0, 0} : (qwk_div){(uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1};
 }
 static bool tr_attn(qw_batch *b) {
-    static const char *const names[2][4][2] = {{{"qwk_attn_w8_f1_d64_q1", "qwk_attn_w8_f1_d64_q2"}, {"qwk_attn_w8_f1_d128_q1", "qwk_attn_w8_f1_d128_q2"}, {"qwk_attn_w8_f1_d192_q1", "qwk_attn_w4_f1_d192_q2"}, {"qwk_attn_w8_f1_d256_q1", "qwk_attn_w4_f1_d256_q2"}},
-                                               {{"qwk_attn_w8_f8_d64_q1", "qwk_attn_w8_f8_d64_q2"}, {"qwk_attn_w8_f8_d128_q1", "qwk_attn_w8_f8_d128_q2"}, {"qwk_attn_w8_f8_d192_q1", "qwk_attn_w4_f8_d192_q2"}, {"qwk_attn_w8_f8_d256_q1", "qwk_attn_w4_f8_d256_q2"}}};
+    static const char *const one[2][4] = {{"qwk_attn_f1_d64_q1", "qwk_attn_f1_d128_q1", "qwk_attn_f1_d192_q1", "qwk_attn_f1_d256_q1"}, {"qwk_attn_f8_d64_q1", "qwk_attn_f8_d128_q1", "qwk_attn_f8_d192_q1", "qwk_attn_f8_d256_q1"}},
+                             *const two[2][2] = {{"qwk_attn_f1_d64_q2", "qwk_attn_f1_d128_q2"}, {"qwk_attn_f8_d64_q2", "qwk_attn_f8_d128_q2"}};
     qw_attn_geo x;
     qwk_attn_args a = {0};
     qw_span in[QW_KV_READS], q, out;
@@ -2576,13 +2579,14 @@ static bool tr_attn(qw_batch *b) {
         !apart_all(b, &ws, "the workspace", QW_KV_READS, in, kv_reads)) return false;
     a.group = (uint32_t)(x.q_heads / x.heads), a.window = x.window > 1 << 30 ? 0 : (uint32_t)x.window, a.grid = attn_grid(b->g);
     a.scale = (x.scale > 0 ? x.scale : 1 / sqrtf((float)x.dim)) * 1.44269504f;
-    // rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode
-    const unsigned qt = cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
-    a.ml = a.part + attn_part_bytes(b->g, x.dim, 2) / 4;
-    a.parts = a.ml + attn_part_bytes(b->g, 2, 2) / 4;
+    // Rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode. 8 slots of 4000 tokens, 24 and 64 of
+    // them, one and two blocks: heads of 64 values, binary16 27.3, 44.9 and 19.8, 29.2 us, Q8_0 20.8, 29.8 and 18.9, 26.7; of 128 27.9, 46.4 and 22.1, 31.2, Q8_0 21.1, 31.1 and 21.2, 27.6; 16 of them (half of
+    // the second empty) 16.3 and 19.5. Larger heads: two blocks need a SIMD's registers for one wave, 30.5 and 33.2, Q8_0 31.5 and 38.5 at 64 of 256 values.
+    const unsigned qt = x.dim <= 128 && cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
+    a.ml = a.part + attn_rows(b->g, x.dim) * (size_t)x.dim;
+    a.parts = a.ml + attn_rows(b->g, x.dim) * 2;
     a.by_group = div_of(a.group), a.by_grid = div_of(a.grid);
-    const char *name = names[x.type == 8][x.dim / 64 - 1][qt - 1];
-    if (!add_launch(b, name, a.grid, name[strlen("qwk_attn_w")] == '8' ? 512 : 256, &a, sizeof a)) return false;
+    if (!add_launch(b, qt == 1 ? one[x.type == 8][x.dim / 64 - 1] : two[x.type == 8][x.dim / 64 - 1], a.grid, QW_WG_ATTN, &a, sizeof a)) return false;
     if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", a.grid, QW_WG_JOIN, &a, sizeof a)) return false;
     b->l[b->nl - 1].gy = 2; // of the pair that a workgroup went on with, and of the one that it began
     return true;

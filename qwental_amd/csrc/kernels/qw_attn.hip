@@ -28,7 +28,7 @@ enum { F16 = 1, Q8 = 8 };
 // result), and qwk_attn_join puts these together in the order of the shares: the same bits every time.
 //
 // Eight waves a workgroup take a share's tiles in turn, each with the next step's units on their way while it works on the last; two workgroups of four a compute unit left twice as much for
-// the join (drafts 32.3 us, not 29.4; one token over 700 tokens 11.9, not 12.1). A wave with two blocks of queries of 192 or 256 values needs all of a SIMD's registers: four waves there.
+// the join (drafts 32.3 us, not 29.4; one token over 700 tokens 11.9, not 12.1).
 //
 // Bound: by the cache's bytes once there are enough of them. 64 slots of 8192 tokens, binary16, 4 heads of 128 values (1.07 GB) 178 us, 5.9 TB/s; one slot of 131072, Q8_0, 2 heads of 256
 // (143 MB) 30 us and 5 for the join; 16 slots of up to 4096, binary16 (78 MB) 17 and 4. Two blocks of queries make Q8_0 instruction-bound (a step, two units of 128 values, is some
@@ -364,8 +364,8 @@ struct Part {
 };
 static_assert(sizeof(Part) == QW_ATTN_PART, "");
 
-template <int TYPE, int D, int QT, int W> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
-    constexpr int U = D <= 128 ? 2 : 1, LD = D + 4, STEPS = 2 / U; // U: units a wave has in hand; a tile is two
+template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
+    constexpr int W = QW_WG_ATTN / 64, U = D <= 128 ? 2 : 1, LD = D + 4, STEPS = 2 / U; // U: units a wave has in hand; a tile is two
     __shared__ float4_t so[W][16 * QT][LD / 4];
     __shared__ float sm[W][16 * QT], sl[W][16 * QT];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -610,12 +610,11 @@ template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args 
     }
 }
 
-#define QW_ATTN(W, TYPE, D, QT, PER) \
-    extern "C" __global__ __launch_bounds__(W * 64, PER) void qwk_attn_w##W##_f##TYPE##_d##D##_q##QT(qwk_attn_args a) { attn_body<TYPE, D, QT, W>(a); }
-QW_ATTN(8, 1, 64, 1, 2) QW_ATTN(8, 8, 64, 1, 2) QW_ATTN(8, 1, 64, 2, 2) QW_ATTN(8, 8, 64, 2, 2)
-QW_ATTN(8, 1, 128, 1, 2) QW_ATTN(8, 8, 128, 1, 2) QW_ATTN(8, 1, 128, 2, 2) QW_ATTN(8, 8, 128, 2, 2)
-QW_ATTN(8, 1, 192, 1, 2) QW_ATTN(8, 8, 192, 1, 2) QW_ATTN(4, 1, 192, 2, 1) QW_ATTN(4, 8, 192, 2, 1)
-QW_ATTN(8, 1, 256, 1, 2) QW_ATTN(8, 8, 256, 1, 2) QW_ATTN(4, 1, 256, 2, 1) QW_ATTN(4, 8, 256, 2, 1)
+#define QW_ATTN(TYPE, D, QT) \
+    extern "C" __global__ __launch_bounds__(QW_WG_ATTN, 2) void qwk_attn_f##TYPE##_d##D##_q##QT(qwk_attn_args a) { attn_body<TYPE, D, QT>(a); }
+QW_ATTN(1, 64, 1) QW_ATTN(8, 64, 1) QW_ATTN(1, 64, 2) QW_ATTN(8, 64, 2)
+QW_ATTN(1, 128, 1) QW_ATTN(8, 128, 1) QW_ATTN(1, 128, 2) QW_ATTN(8, 128, 2)
+QW_ATTN(1, 192, 1) QW_ATTN(8, 192, 1) QW_ATTN(1, 256, 1) QW_ATTN(8, 256, 1)
 #define QW_JOIN(QT) extern "C" __global__ __launch_bounds__(QW_WG_JOIN) void qwk_attn_join_q##QT(qwk_attn_args a) { join_body<QT>(a); }
 QW_JOIN(1)
 QW_JOIN(2)

@@ -4,6 +4,7 @@
 
 #define QW_UNIT 16u           /* tokens of a unit: what the cache's layout is made of */
 #define QW_ATTN_TILE 32u      /* tokens by which the work is shared out */
+#define QW_WG_ATTN 512u       /* eight waves, each with tiles of its own */
 #define QW_WG_JOIN 256u
 #define QW_WG_KV 256u
 #define QW_KV_SLOTS_MAX 256u  /* a thread of a workgroup for each */

@@ -298,3 +298,10 @@ def test_angles_near_zero(gpu, dev, freq):
     xb = dev.up(x)
     dev.run(q.KvWrite(dev.cache(c), dev.step(s), 1, xb, out, xb, xb, q.Rope(64, [32], dev.up(np.full(32, freq)), dev.up(pos))))
     assert np.array_equal(out.read(dtype=np.float16).reshape(x.shape), turned(x, pos, np.full(32, freq), [32], False))
+
+
+@pytest.mark.parametrize("rot", ["halves", "adjacent", "part", "none"])
+@pytest.mark.parametrize("shape", [(F16, 2, 16, 64, 16, [600], [600]), (Q8, 4, 32, 128, 64, [1400], [3001]), (Q8, 1, 5, 256, 32, [1500, 1, 703], [1507, 1, 703]), (F16, 3, 3, 192, 16, [300, 900], [300, 1000])])
+def test_many_rows_into_the_cache_and_back(gpu, dev, shape, rot):
+    """Several heads a wave."""
+    test_rows_into_the_cache_and_back(gpu, dev, shape, rot)
