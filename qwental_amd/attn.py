@@ -72,7 +72,7 @@ class _Call:
     def __call__(self, batch):
         if self.f is None:
             self.f = getattr(batch.L, self.name)
-        batch.__dict__.setdefault("keep", []).append(self)  # buffers of a call that nobody else holds last as long as the batch
+        batch.keep.append(self)  # buffers of a call that nobody else holds last as long as the batch
         if not self.f(batch.b, *self.args):
             raise RuntimeError("%s failed: %s" % (self.name, batch.gpu.last_error()))
 

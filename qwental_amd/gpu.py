@@ -253,7 +253,7 @@ class MoeLayer:
 
 class Batch:
     def __init__(self, gpu, concurrent=False):
-        self.gpu, self.L = gpu, gpu.L
+        self.gpu, self.L, self.keep = gpu, gpu.L, []
         self.b = self.L.qw_batch_begin(gpu.g, concurrent)
 
     def kernel(self, k):
@@ -285,7 +285,7 @@ class StreamBatch(Batch):
     with statement it ends at the block's end, or is dropped where the block raises."""
 
     def __init__(self, gpu, stream=None):
-        self.gpu, self.L = gpu, gpu.L
+        self.gpu, self.L, self.keep = gpu, gpu.L, []
         self.b = self.L.qw_hip_stream_begin(gpu.g, stream)
         if not self.b:
             raise RuntimeError(gpu.last_error())
