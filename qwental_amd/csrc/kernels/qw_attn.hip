@@ -589,9 +589,17 @@ template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args 
         float top = neg, sum = 0;
         float4_t o = {0, 0, 0, 0};
         if (sub < lanes)
-            for (uint32_t w = p.w0 + sub; w <= p.w1; w += lanes) {
-                const size_t at = ((size_t)w * 2 + (w == p.w0)) * 16 * QT + row;
-                add(top, sum, o, a.ml[at * 2], a.ml[at * 2 + 1], *(const float4_t *)(a.part + at * a.c.dim + at4 * 4));
+            for (uint32_t w = p.w0 + sub; w <= p.w1; w += 4 * lanes) { // four at a time: their loads go out together (one behind the other: 6.4 us for 8 shares of 32 rows of 128 values)
+                float m[4], l[4];
+                float4_t v[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    const uint32_t x = min(w + i * lanes, p.w1);
+                    const size_t at = ((size_t)x * 2 + (x == p.w0)) * 16 * QT + row;
+                    m[i] = a.ml[at * 2], l[i] = a.ml[at * 2 + 1], v[i] = *(const float4_t *)(a.part + at * a.c.dim + at4 * 4);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) add(top, sum, o, w + i * lanes <= p.w1 ? m[i] : neg, l[i], v[i]);
             }
         while (lanes > 1) {
             const uint32_t half = (lanes + 1) / 2;
