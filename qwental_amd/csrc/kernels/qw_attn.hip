@@ -32,7 +32,7 @@ enum { F16 = 1, Q8 = 8 };
 //
 // Bound: by the cache's bytes once there are enough of them. 64 slots of 8192 tokens, binary16, 4 heads of 128 values (1.07 GB) 178 us, 5.9 TB/s; one slot of 131072, Q8_0, 2 heads of 256
 // (143 MB) 30 us and 5 for the join; 16 slots of up to 4096, binary16 (78 MB) 17 and 4. Two blocks of queries make Q8_0 instruction-bound (a step, two units of 128 values, is some
-// 500 vector and 64 matrix instructions): 12 slots of 45 rows over 6001 tokens 23 us for 55 MB, of which 4 are gone before the first unit arrives. One token over 700: 8.4 us, five
+// 500 vector and 64 matrix instructions): 12 slots of 45 rows over 6001 tokens 24 us for 55 MB, of which 4 are gone before the first unit arrives. One token over 700: 8.5 us, five
 // dependent round trips to memory and the launch.
 
 struct Slot { int n, len, first; }; // rows, tokens, first row
@@ -564,7 +564,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
 }
 
 // Results of pairs that several workgroups share, put together by as many: of the pair's results, workgroup w takes its part, and its threads share
-// what the others left of them. A pair of 128 shares (8 rows of 256 values, 131072 tokens) costs a thread a load or two, as one of two shares does. 4 to 6 us: two round trips and the launch
+// what the others left of them. A pair of 128 shares (8 rows of 256 values, 131072 tokens) costs a thread a load or two, as one of two shares does. 4 to 5 us: two round trips and the launch
 // (one workgroup a pair took 28 for that one). A launch of its own, because the workgroup that comes last would have to be told apart by a counter, and the workspace need not be cleared.
 template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args &a) {
     __shared__ float4_t so[QW_WG_JOIN];
