@@ -190,7 +190,7 @@ template <int TYPE, int D, int QT, int U> struct Attn {
     const uint32_t lane;
     half8_t q[QT][D / 32];
     float4_t acc[QT][D / 32][2]; // result: value 32 b + 8 (lane >> 4) + 2 i + c of query lane & 15
-    float m[QT], l[QT];          // reference (log2) and this lane's part of the sum
+    float m[QT], l[QT];          // the largest score so far (as the product leaves it, not yet times the scale) and this lane's part of the sum
     int hi[QT], lo[QT];          // tokens [lo, hi) that the lane's query sees
     UnitData<TYPE, D> K[U], V[U];
 
@@ -250,22 +250,21 @@ template <int TYPE, int D, int QT, int U> struct Attn {
             for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) top = fmaxf(top, p[t][i][j]);
-            top *= a.scale;
             if (__any(top > m[t])) { // (as a rule in a wave's first steps only)
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float now = fmaxf(m[t], top), f = m[t] == neg ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
+                const float now = fmaxf(m[t], top), f = m[t] == neg ? 0.f : __builtin_amdgcn_exp2f((m[t] - now) * a.scale);
                 m[t] = now;
                 l[t] *= f;
 #pragma unroll
                 for (int b = 0; b < D / 32; b++) acc[t][b][0] *= f, acc[t][b][1] *= f;
             }
-            const float ref = m[t] == neg ? 0.f : TOP - m[t];
+            const float ref = m[t] == neg ? 0.f : m[t]; // (taken off before the scale: the largest weight is 2^14 then, however large its score)
 #pragma unroll
             for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    p[t][i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i][j], a.scale, ref));
+                    p[t][i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i][j] - ref, a.scale, TOP));
                     l[t] += p[t][i][j];
                 }
         }
@@ -538,7 +537,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
             for (int w = 0; w < W; w++) top = fmaxf(top, f[w] = sm[w][row]);
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                f[w] = f[w] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(f[w] - top);
+                f[w] = f[w] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((f[w] - top) * a.scale);
                 sum += sl[w][row] * f[w];
             }
             const int j = by(a.by_group, mr);
@@ -579,7 +578,7 @@ template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args 
     // one with what another left
     const auto add = [&](float &top, float &sum, float4_t &o, float mw, float lw, float4_t ow) {
         if (mw == neg) return;
-        const float now = fmaxf(top, mw), f = top == neg ? 0.f : __builtin_amdgcn_exp2f(top - now), fw = __builtin_amdgcn_exp2f(mw - now);
+        const float now = fmaxf(top, mw), f = top == neg ? 0.f : __builtin_amdgcn_exp2f((top - now) * a.scale), fw = __builtin_amdgcn_exp2f((mw - now) * a.scale);
         top = now, sum = sum * f + lw * fw, o = o * f + ow * fw;
     };
     for (uint32_t o0 = k * all / np; o0 < o1; o0 += QW_WG_JOIN) { // quads of results [o0, o1), at most as many as there are threads

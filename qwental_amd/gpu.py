@@ -292,6 +292,8 @@ class StreamBatch(Batch):
 
     def end(self):
         b, self.b = self.b, None
+        if not b or not self.gpu.g:
+            raise RuntimeError("this recorder has ended, or its device is closed")
         if not self.L.qw_hip_stream_end(b):
             raise RuntimeError("GPU launches failed: " + self.gpu.last_error())
 

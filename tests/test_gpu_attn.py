@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import qwental_amd as q
-from attn_helpers import F16, Q8, Cache, Step, attention, turned
+from attn_helpers import F16, Q8, Cache, Step, attention, scale_places, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -70,6 +70,9 @@ SHAPES = [  # type, kv heads, query heads, dim, page, rows a slot, tokens a slot
     (F16, 2, 2, 256, 256, [33, 1], [40, 257]),
     (Q8, 1, 40, 192, 64, [2, 2], [2, 65]),
     (F16, 8, 64, 64, 16, [1, 0, 2], [16, 5, 48]),
+    (F16, 256, 256, 64, 16, [1, 1], [20, 3]),      # the most heads there are
+    (Q8, 1, 1024, 64, 32, [1, 2], [33, 70]),
+    (F16, 1, 2, 64, 4096, [1, 2], [5000, 10]),     # pages larger than what they hold
 ]
 
 
@@ -305,3 +308,61 @@ def test_angles_near_zero(gpu, dev, freq):
 def test_many_rows_into_the_cache_and_back(gpu, dev, shape, rot):
     """Several heads a wave."""
     test_rows_into_the_cache_and_back(gpu, dev, shape, rot)
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
+@pytest.mark.parametrize("scale", [1.0, 1e5, 1e12, 1e30])
+def test_scores_of_any_size(gpu, dev, kind, scale):
+    """Whole numbers, so that scores are exact and their differences 2 at least: all weight lies on the largest, or on those that share it, whatever it is times the scale. (At scale 1 the others have
+    e^-2 and less of it: as everywhere.) Results are off by their rounding, 2^-11, and what 4096 such sums lose, 2^-12 of the largest value."""
+    rng = np.random.default_rng(37)
+    s = Step(rng, [2, 1], [700, 90], 32)
+    c = Cache(kind, 2, 64, 32, s.pages, fill=0xffff)
+    for i, n in enumerate(s.len):
+        for t in range(int(n)):
+            c.put(s.table, i, t, (2 * rng.integers(-63, 64, (2, 64)) + 1).astype(np.float16), rng.standard_normal((2, 64)).astype(np.float16))
+    if kind == Q8:  # scales of the keys: 1
+        for values, w in ((False, 1.0),):
+            at = scale_places(64, values)
+            for b in range(2):
+                c.raw[..., at + b] = np.frombuffer(np.float16(w).tobytes(), np.uint8)[b]
+    qr = (2 * rng.integers(-3, 4, (3, 8, 64))).astype(np.float16)
+    if scale == 1.0:
+        qr = (qr / 4096).astype(np.float16)
+    out, ws = dev.new(qr.nbytes), dev.new(q.attn_ws_bytes(gpu, 64))
+    dev.run(q.Attn(dev.cache(c), dev.step(s), 8, dev.up(qr), out, ws, scale=scale))
+    got = out.read(dtype=np.float16).reshape(qr.shape).astype(np.float64)
+    for row, slot, token in s.rows_of():
+        k, v = c.get(s.table, slot, range(token + 1))
+        x = np.einsum("hgd,thd->hgt", qr[row].astype(np.float64).reshape(2, 4, 64), k)
+        p = np.exp(np.maximum((x - x.max(-1, keepdims=True)) * scale, -1e4))
+        want = np.einsum("hgt,thd->hgd", p / p.sum(-1, keepdims=True), v).reshape(8, 64)
+        assert (np.abs(got[row] - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -12 * np.abs(v).max()).all()
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
+def test_tokens_beyond_two_to_the_29(gpu, dev, kind):
+    """The last tokens of slots of 2^29 and 2^30, of which two pages each are there: rows in, out, and attention in a window."""
+    rng = np.random.default_rng(41)
+    page, window = 65536, 150
+    s = Step.__new__(Step)
+    s.n, s.len, s.rows, s.pages, s.max_pages = np.array([2, 3]), np.array([(1 << 29) + 70, (1 << 30) - 1]), 5, 4, 1 << 14
+    s.first, s.table = np.array([0, 2, 5]), np.full((2, 1 << 14), 0xffffffff, np.uint32)
+    s.table[0, 8191:8193] = 2, 0
+    s.table[1, 16382:] = 1, 3
+    c = Cache(kind, 2, 64, page, 4, fill=0xffff)
+    for i, n in enumerate(s.len):
+        for t in range(int(n) - 300, int(n)):
+            c.put(s.table, i, t, *rng.standard_normal((2, 2, 64)).astype(np.float16))
+    k, v, qr = rows(rng, 5, 2, 64), rows(rng, 5, 2, 64), rows(rng, 5, 8, 64)
+    kc, st, qb, back = dev.cache(c), dev.step(s), dev.up(qr), [dev.new(k.nbytes) for _ in range(2)]
+    out, ws = dev.new(qr.nbytes), dev.new(q.attn_ws_bytes(gpu, 64))
+    dev.run(q.KvWrite(kc, st, 0, None, None, dev.up(k), dev.up(v)), q.KvRead(kc, st, *back), q.Attn(kc, st, 8, qb, out, ws, window=window))
+    for row, slot, token in s.rows_of():
+        c.put(s.table, slot, token, k[row], v[row])
+    assert np.array_equal(kc.keep.read(), c.raw.ravel())
+    for row, slot, token in s.rows_of():
+        for got, want in zip(back, c.get(s.table, slot, [token])):
+            assert np.array_equal(got.read(dtype=np.float16).reshape(k.shape)[row], want[0].astype(np.float16))
+    want, tol = attention(c, s, qr, 0.125, window)
+    assert (np.abs(out.read(dtype=np.float16).reshape(qr.shape) - want) <= tol).all()

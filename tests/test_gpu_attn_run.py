@@ -316,3 +316,23 @@ def test_recorder_is_given_back(gpu, dev):
         gpu.view(np.zeros(64).ctypes.data, 64)
     with pytest.raises(RuntimeError, match="beyond"):
         gpu.view(t.ws.data_ptr(), 1 << 40)
+
+
+def test_captured_at_a_devices_first_use():
+    """Nothing has to be called before a capture; views outlive the device."""
+    rng = np.random.default_rng(60)
+    g = q.Gpu()
+    t = Torch(g, rng, Q8, [1, 1], [40, 3], [60, 20], D=192, H=1, V=9000)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.run(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        t.feed(rng)
+        graph.replay()
+        torch.cuda.synchronize()
+        t.verify()
+    late = g.stream(None)
+    g.close()
+    with pytest.raises(RuntimeError, match="closed"):
+        late.end()
