@@ -770,13 +770,13 @@ template <int TYPE, uint32_t C> __device__ __forceinline__ void kv_write_body(co
                 if (2 * d[k] >= D) continue;
                 uint32_t r = x[n][k];
                 if (2 * d[k] < a.rot) { // (an even number: both values turn or neither)
-                    // In 32 bits with a bound on what that is off by: the factors and one product half a step of 24 bits each, the sum half a step of its own. Where both ends of the interval
-                    // round to the same half, that is the result; the others, one value in a thousand or so (and zeros, whose sign the bound does not tell), are made in 64 bits.
+                    // In 32 bits with a bound on what that is off by: the factors and one product half a step of 24 bits each, the sum half a step of its own, and so have the interval's ends:
+                    // 2^-24 of |u c| three times, of |w s| twice, of the sum once more, and 2^-120 for factors below 2^-126. Where both ends round to the same half, that is the result; the others, one value in a thousand or so (and zeros, whose sign the bound does not tell), are made in 64 bits.
                     uint32_t lo = 0, hi = 0;
 #pragma unroll
                     for (uint32_t e = 0; e < 2; e++) {
                         const float u = half_of((uint16_t)(r >> 16 * e)), w = half_of((uint16_t)(y[n][k] >> 16 * e)), uc = u * (float)cs[k][e], ws = w * (float)sn[k][e];
-                        const float sum = __builtin_fmaf(w, (float)sn[k][e], uc), off = __builtin_fmaf(__builtin_fabsf(uc) + __builtin_fabsf(ws), 0x3.1p-24f, 0x1p-120f);
+                        const float sum = __builtin_fmaf(w, (float)sn[k][e], uc), off = __builtin_fmaf(__builtin_fabsf(uc) + __builtin_fabsf(ws), 0x4.2p-24f, 0x1p-120f);
                         lo |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(sum - off)) << 16 * e, hi |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(sum + off)) << 16 * e;
                     }
                     if (__builtin_expect(lo != hi, 0))
