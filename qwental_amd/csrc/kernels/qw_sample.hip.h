@@ -285,7 +285,6 @@ struct SampleFast {
     uint32_t count[QW_SAMPLE_BINS], fine_count[FEW], key[LIST], id[LIST], few_key[FEW], few_id[FEW], pos[TILES], from[TILES], many[TILES], shift[TILES];
     int off[TILES]; // bins that a tile's first lies below the row's; shift: of its weights, by octaves
     uint16_t starts[NEAR_TILES * (QW_SAMPLE_BINS + 1)]; // of up to so many tiles, and the tokens of their first bins
-    uint32_t near_key[NEAR], near_id[NEAR];
     uint32_t n, few, pick, cut_key, cut_id, slow, which;
     u64 before_n, before_w;
 };
@@ -348,14 +347,23 @@ struct FastSampler {
         }
         __syncthreads();
         if (s.n > LIST) return false;
-        for (uint32_t tile = t / 32; tile < a.tiles; tile += QW_WG_SAMPLE / 32)
-            for (uint32_t i = t % 32; i < s.many[tile]; i += 32) {
-                const uint32_t at = s.from[tile] + i;
-                uint32_t id, key;
-                if (at < near) id = s.near_id[tile * near + at], key = s.near_key[tile * near + at];
-                else id = tile * QW_SAMPLE_TILE + a.order[(first_tile + tile) * QW_SAMPLE_TILE + at], key = key_of(l[id]);
-                s.id[s.pos[tile] + i] = id, s.key[s.pos[tile] + i] = key;
+        // as many threads a tile as there are, four tokens a thread at once (two dependent loads each: one token after the other, by 32 threads, it was most of a wide border's 7 us)
+        const uint32_t log2 = a.tiles > 1 ? 32 - (uint32_t)__builtin_clz(a.tiles - 1) : 0, tile = t >> (10 - log2), lanes = QW_WG_SAMPLE >> log2, mine = t & (lanes - 1);
+        static_assert(QW_WG_SAMPLE == 1 << 10 && TILES <= QW_WG_SAMPLE, "");
+        if (tile < a.tiles) {
+            const uint32_t many = s.many[tile], from = s.from[tile], pos = s.pos[tile];
+            const uint16_t *order = a.order + (first_tile + tile) * QW_SAMPLE_TILE;
+            for (uint32_t i = mine; i < many; i += 4 * lanes) {
+                uint32_t id[4], key[4];
+#pragma unroll
+                for (uint32_t n = 0; n < 4; n++) id[n] = tile * QW_SAMPLE_TILE + order[from + min(i + n * lanes, many - 1)];
+#pragma unroll
+                for (uint32_t n = 0; n < 4; n++) key[n] = key_of(l[id[n]]);
+#pragma unroll
+                for (uint32_t n = 0; n < 4; n++)
+                    if (i + n * lanes < many) s.id[pos + i + n * lanes] = id[n], s.key[pos + i + n * lanes] = key[n];
             }
+        }
         __syncthreads();
         loaded = bin;
         return true;
@@ -508,14 +516,12 @@ __device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t ro
     __syncthreads();
     // A thread a bin of every fourth tile; four tiles' loads at once, wanted or not (one after the other behind a look at the bin's count: 20 us of 31).
     constexpr uint32_t EVERY = QW_WG_SAMPLE / QW_SAMPLE_BINS;
-    // Beside them the first tokens of every tile's order, a thread each: a border among the row's first some hundred tokens then costs no round trips of its own.
+    // Beside them the first tokens of every tile's order, a thread each: a row of which a filter leaves few needs only their logits then.
     const uint32_t near = a.tiles <= NEAR / 64 ? 64 : a.tiles <= NEAR_TILES ? NEAR / NEAR_TILES : 0;
-    uint32_t near_id = 0, near_key = 0;
+    uint32_t near_id = 0;
     if (near && t < near * a.tiles) {
-        const uint32_t tile = t / near, i = t % near, in = min(a.vocab - tile * QW_SAMPLE_TILE, QW_SAMPLE_TILE);
-        const uint32_t at = i < in ? a.order[(first_tile + tile) * QW_SAMPLE_TILE + i] : 0;
-        near_id = tile * QW_SAMPLE_TILE + min(at, in - 1); // (a tile without bins has left no order)
-        near_key = key_of(l[near_id]);
+        const uint32_t tile = t / near, i = t % near;
+        if (i < min(a.vocab - tile * QW_SAMPLE_TILE, QW_SAMPLE_TILE)) near_id = tile * QW_SAMPLE_TILE + a.order[(first_tile + tile) * QW_SAMPLE_TILE + i]; // (a tile without bins has left none)
     }
     const uint32_t bin = t % QW_SAMPLE_BINS;
     for (uint32_t from = t / QW_SAMPLE_BINS; from < a.tiles; from += 4 * EVERY) {
@@ -545,7 +551,6 @@ __device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t ro
             if (v) atomicAdd(&s.weight[b], v);
         }
     }
-    if (near) s.near_id[t] = near_id, s.near_key[t] = near_key;
     __syncthreads();
     FastSampler f{s, a, l, weigh, first_tile, g, near};
     uint32_t cut_key = 0, cut_id = ~0u; // the last token kept
@@ -571,7 +576,8 @@ __device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t ro
                 if (end > near) s.slow = 1;
                 else if (i < end) {
                     const uint32_t k = atomicAdd(&s.few, 1u);
-                    s.few_key[k] = near_key, s.few_id[k] = near_id, s.few_weight[k] = weigh(of_key(near_key));
+                    const float x = l[near_id];
+                    s.few_key[k] = key_of(x), s.few_id[k] = near_id, s.few_weight[k] = weigh(x);
                 }
             }
             __syncthreads();
@@ -635,40 +641,31 @@ __device__ bool sample_fast(SampleFast &s, const qwk_sample_args &a, uint32_t ro
                 if (below <= at && at < below + n[k]) s.which = t * (TILES / 64) + k, s.below = at - below;
     }
     __syncthreads();
-    // in the tile that the draw falls into: 64 tokens a wave at a time, then one of them
+    // in the tile that the draw falls into: a wave's stretch of it, then, by that wave alone, 64 tokens at a time
     constexpr uint32_t K = QW_SAMPLE_TILE / QW_WG_SAMPLE, WAVES = QW_WG_SAMPLE / 64;
-    const uint32_t base = s.which * QW_SAMPLE_TILE;
-    u64 w[K], up[K];
+    const uint32_t base = s.which * QW_SAMPLE_TILE + wave * (K * 64) + lane;
+    u64 w[K], sum = 0;
     float x[K];
 #pragma unroll
-    for (uint32_t k = 0; k < K; k++) x[k] = l[min(base + k * QW_WG_SAMPLE + t, a.vocab - 1)];
+    for (uint32_t k = 0; k < K; k++) x[k] = l[min(base + k * 64, a.vocab - 1)];
 #pragma unroll
-    for (uint32_t k = 0; k < K; k++) {
-        const uint32_t id = base + k * QW_WG_SAMPLE + t;
-        w[k] = id < a.vocab ? weight(key_of(x[k]), id) : 0, up[k] = wave_up(w[k]);
-        if (lane == 63) s.fine_weight[k * WAVES + wave] = up[k];
-    }
+    for (uint32_t k = 0; k < K; k++) sum += w[k] = base + k * 64 < a.vocab ? weight(key_of(x[k]), base + k * 64) : 0;
+    sum = of_lane(wave_up(sum), 63);
+    if (lane == 0) s.fine_weight[wave] = sum;
     __syncthreads();
-    static_assert(K * WAVES == 128, "two a lane");
-    u64 whole = 0, mine_below[K] = {};
-    {
-        const u64 n0 = s.fine_weight[lane * 2], n1 = s.fine_weight[lane * 2 + 1], u = wave_up(n0 + n1);
-        whole = of_lane(u, 63);
-#pragma unroll
-        for (uint32_t k = 0; k < K; k++) { // what lies before this wave's k-th group
-            const uint32_t at = k * WAVES + wave;
-            mine_below[k] = of_lane(u, (int)(at / 2)) - of_lane(at % 2 ? n1 : n0 + n1, (int)(at / 2));
-        }
-    }
+    const u64 up = wave_up(lane < WAVES ? s.fine_weight[lane] : 0), whole = of_lane(up, 63);
     if (!whole) return false;
     const u64 at = min((u64)s.below, whole - 1); // (the tile's bins and its tokens may add up to some units' difference)
+    u64 c = wave ? of_lane(up, (int)wave - 1) : 0;
+    if (at < c || at >= c + sum) return true;
 #pragma unroll
     for (uint32_t k = 0; k < K; k++) {
-        const u64 c = mine_below[k] + up[k];
-        if (c - w[k] <= at && at < c) {
-            a.ids[row] = base + k * QW_WG_SAMPLE + t;
+        const u64 end = c + wave_up(w[k]);
+        if (end - w[k] <= at && at < end) {
+            a.ids[row] = base + k * 64;
             if (a.probs) a.probs[row] = (float)((double)w[k] / (double)s.all);
         }
+        c = of_lane(end, 63);
     }
     return true;
 }
