@@ -304,24 +304,28 @@ struct FastSampler {
         __syncthreads();
         if (threadIdx.x < 64) {
             constexpr int K = N / 64;
-            u64 w = 0, n = 0;
+            const int first = (int)threadIdx.x * K;
+            u64 w = 0, n = 0, ws[K];
+            uint32_t ns[K];
             int last = -1;
+#pragma unroll
             for (int k = 0; k < K; k++) {
-                w += weight[threadIdx.x * K + k], n += count[threadIdx.x * K + k];
-                if (count[threadIdx.x * K + k]) last = (int)threadIdx.x * K + k;
+                w += ws[k] = weight[first + k], n += ns[k] = count[first + k];
+                if (ns[k]) last = first + k;
             }
             const u64 uw = wave_up(w), un = wave_up(n);
             const u64 hit = __ballot((weights ? uw : un) >= want && n), any = __ballot(last >= 0);
             const uint32_t lane = hit ? (uint32_t)__builtin_ctzll(hit) : any ? 63u - (uint32_t)__builtin_clzll(any) : 0;
             if (threadIdx.x == lane) {
                 u64 bw = uw - w, bn = un - n;
-                int k = 0;
-                while ((int)lane * K + k < last) {
-                    const u64 ww = weight[lane * K + k], nn = count[lane * K + k];
-                    if ((weights ? bw + ww : bn + nn) >= want && nn) break;
-                    bw += ww, bn += nn, k++;
+                int at = first;
+                bool on = true;
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    on = on && first + k < last && !((weights ? bw + ws[k] : bn + ns[k]) >= want && ns[k]);
+                    if (on) bw += ws[k], bn += ns[k], at++;
                 }
-                s.pick = lane * K + (uint32_t)k, s.before_w = bw, s.before_n = bn;
+                s.pick = (uint32_t)at, s.before_w = bw, s.before_n = bn;
             }
         }
         __syncthreads();
