@@ -314,7 +314,8 @@ class StreamBatch(Batch):
             self.drop()
 
     def __del__(self):
-        self.drop()
+        if self.b:
+            self.drop()
 
 
 class View(Buf):
