@@ -89,11 +89,15 @@ class KvWrite(_Call):
 
 
 class KvRead(_Call):
+    """The rows' keys and values (binary16) out of the cache. strides: values from row to row of k, v (0: dense)."""
+
     def __init__(self, cache, step, k, v, strides=(0, 0)):
         super().__init__("qw_kv_read", (cache, step, k, v), cache.c, step.c, _rows(k, strides[0]), _rows(v, strides[1]))
 
 
 class Attn(_Call):
+    """out = the attention of rows q over their slots' tokens (binary16 [rows][q_heads][dim]); scale 0: 1 / sqrt(dim); window 0: all tokens. ws: attn_ws_bytes of device memory, one call's at a time."""
+
     def __init__(self, cache, step, q_heads, q, out, ws, scale=0.0, window=0, strides=(0, 0)):
         super().__init__("qw_attn", (cache, step, q, out, ws), cache.c, step.c, q_heads, _rows(q, strides[0]), _rows(out, strides[1]), scale, window, _at(ws))
 

@@ -173,6 +173,56 @@ def test_steps_of_a_model(gpu, oracle, dev, kind):
     path.close()
 
 
+@pytest.mark.parametrize("kind", [F16, Q8])
+def test_buffers_with_a_host_side(gpu, dev, kind):
+    """Everything but the cache and the workspaces in buffers that the host sees; written through their views, read there when the batch has ended."""
+    rng = np.random.default_rng(70 + kind)
+    H, G, D, page, V = 2, 4, 64, 32, 700
+    s = Step(rng, [2, 1], [40, 7], page, rows=5)  # two rows of no slot
+    c = filled(rng, kind, H, D, page, s)
+    kc = dev.cache(c)
+    keep = []
+
+    def host(a):
+        keep.append(gpu.buf(a.nbytes))
+        keep[-1].fill(a)
+        return keep[-1]
+
+    first, lens, table = (host(a.astype(np.uint32)) for a in (s.first, s.len, s.table))
+    st = q.KvStep(2, 5, s.max_pages, first, lens, table)
+    shapes = [(5, H * G, D), (5, H, D), (5, H, D)]
+    data = [rows(rng, *sh) for sh in shapes]
+    qb, kb, vb = (host(a) for a in data)
+    out, k2, v2, ids, probs = (host(np.full(n, 0x1234, np.uint16)) for n in (5 * H * G * D, 5 * H * D, 5 * H * D, 10, 10))
+    logits, params, u = host(model_like(rng, 5, V)), host(np.array([(0.8, 0.9, 0.0, 30)] * 5, ROW)), host(rng.random(5).astype(np.float32))
+    ws, sws = dev.new(q.attn_ws_bytes(gpu, D)), dev.new(q.sample_ws_bytes(gpu, 5, V))
+    for step in range(3):
+        b = gpu.batch()
+        q.KvWrite(kc, st, 0, None, None, kb, vb)(b)
+        q.KvRead(kc, st, k2, v2)(b)
+        q.Attn(kc, st, H * G, qb, out, ws)(b)
+        q.Sample(5, V, logits, params, u, ids, probs, sws)(b)
+        b.end()
+        for row, slot, token in s.rows_of():
+            c.put(s.table, slot, token, data[1][row], data[2][row])
+            for got, want in zip((k2, v2), c.get(s.table, slot, [token])):
+                assert np.array_equal(got.view(np.float16).reshape(5, H, D)[row], want[0].astype(np.float16))
+        want, tol = attention(c, s, data[0], D ** -0.5)
+        got = out.view(np.float16).reshape(5, H * G, D)
+        assert (np.abs(got[:3] - want[:3]) <= tol[:3]).all() and (out.view(np.uint16).reshape(5, -1)[3:] == 0x1234).all() and (k2.view(np.uint16).reshape(5, -1)[3:] == 0x1234).all()
+        for i in range(5):
+            token, p, near, _ = drawn(logits.view(np.float32).reshape(5, V)[i], params.view(ROW)[i], float(u.view(np.float32)[i]))
+            assert near < 2.0 ** -20 or (ids.view(np.uint32)[i] == token and abs(probs.view(np.float32)[i] - p) < 1e-5)
+        s.len = s.len + 1  # the next step, through the shadows
+        lens.fill(s.len.astype(np.uint32))
+        data = [rows(rng, *sh) for sh in shapes]
+        for buf, a in zip((qb, kb, vb), data):
+            buf.fill(a)
+        logits.fill(model_like(rng, 5, V))
+    for b in keep:
+        b.free()
+
+
 # ---------------------------------------------------------------- a stream and tensors of the caller's
 class Torch:
     """A step of a captured or eager program: cache, rows, tokens, all torch's."""
