@@ -2559,8 +2559,8 @@ static qwk_div div_of(uint32_t d) {
     return d <= 1 ? (qwk_div){0, 0} : (qwk_div){(uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1};
 }
 static bool tr_attn(qw_batch *b) {
-    static const char *const one[2][4] = {{"qwk_attn_f1_d64_q1", "qwk_attn_f1_d128_q1", "qwk_attn_f1_d192_q1", "qwk_attn_f1_d256_q1"}, {"qwk_attn_f8_d64_q1", "qwk_attn_f8_d128_q1", "qwk_attn_f8_d192_q1", "qwk_attn_f8_d256_q1"}},
-                             *const two[2][2] = {{"qwk_attn_f1_d64_q2", "qwk_attn_f1_d128_q2"}, {"qwk_attn_f8_d64_q2", "qwk_attn_f8_d128_q2"}};
+#define QW_ATTN_NAMES(T, S) {{"qwk_attn_f" T "_d64_q1" S, "qwk_attn_f" T "_d128_q1" S, "qwk_attn_f" T "_d192_q1" S, "qwk_attn_f" T "_d256_q1" S}, {"qwk_attn_f" T "_d64_q2" S, "qwk_attn_f" T "_d128_q2" S}}
+    static const char *const names[2][2][2][4] = {{QW_ATTN_NAMES("1", ""), QW_ATTN_NAMES("8", "")}, {QW_ATTN_NAMES("1", "_s"), QW_ATTN_NAMES("8", "_s")}};
     qw_attn_geo x;
     qwk_attn_args a = {0};
     qw_span in[QW_KV_READS], q, out;
@@ -2582,11 +2582,15 @@ static bool tr_attn(qw_batch *b) {
     // Rows x query heads of a head that a workgroup takes at once: 16 fit the matrix instruction; a second block of them shares what a unit costs to load and decode. 8 slots of 4000 tokens, 24 and 64 of
     // them, one and two blocks: heads of 64 values, binary16 27.3, 44.9 and 19.8, 29.2 us, Q8_0 20.8, 29.8 and 18.9, 26.7; of 128 27.9, 46.4 and 22.1, 31.2, Q8_0 21.1, 31.1 and 21.2, 27.6; 16 of them (half of
     // the second empty) 16.3 and 19.5. Larger heads: two blocks need a SIMD's registers for one wave, 30.5 and 33.2, Q8_0 31.5 and 38.5 at 64 of 256 values.
-    const unsigned qt = x.dim <= 128 && cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group > 16 ? 2 : 1;
+    const unsigned rows = cdiv((unsigned)x.rows, (unsigned)x.slots) * a.group, qt = x.dim <= 128 && rows > 16 ? 2 : 1;
+    // Past the caches where a slot's rows are one block, so that no second one reads its units again, and the slots may have more of them than caches keep from one call to the next: 64 slots of 8192 tokens
+    // (1.07 GB) 189.7 -> 168.8 us, one of 131072 (143 MB) 37.9 -> 35.3, 16 of up to 4096 (78 MB, with other calls between) 24.2 -> 22.5, 32 of up to 500 (35 MB) 12.9 -> 13.3; with several blocks 40.2 -> 45.5.
+    const uint64_t most = (uint64_t)x.slots * (uint64_t)x.max_pages, units = (most < (uint64_t)x.pages ? most : (uint64_t)x.pages) * a.c.page_bytes;
+    const bool stream = rows <= 16 * qt && units >= 64u << 20;
     a.ml = a.part + attn_rows(b->g, x.dim) * (size_t)x.dim;
     a.parts = a.ml + attn_rows(b->g, x.dim) * 2;
     a.by_group = div_of(a.group), a.by_grid = div_of(a.grid);
-    if (!add_launch(b, qt == 1 ? one[x.type == 8][x.dim / 64 - 1] : two[x.type == 8][x.dim / 64 - 1], a.grid, QW_WG_ATTN, &a, sizeof a)) return false;
+    if (!add_launch(b, names[stream][x.type == 8][qt - 1][x.dim / 64 - 1], a.grid, QW_WG_ATTN, &a, sizeof a)) return false;
     if (!add_launch(b, qt == 1 ? "qwk_attn_join_q1" : "qwk_attn_join_q2", a.grid, QW_WG_JOIN, &a, sizeof a)) return false;
     b->l[b->nl - 1].gy = 2; // of the pair that a workgroup went on with, and of the one that it began
     return true;

@@ -135,13 +135,15 @@ __device__ __forceinline__ half4_t codes(uint32_t w) {
     return half4_t{lo.x, lo.y, hi.x, hi.y};
 }
 
+// STREAM: past the caches, for what nobody reads again before the whole cache has gone by.
+template <bool STREAM> __device__ __forceinline__ uint4_t sixteen(const uint8_t *p) { return STREAM ? __builtin_nontemporal_load((const uint4_t *)p) : *(const uint4_t *)p; }
 template <int TYPE, int D> struct UnitData; // a lane's share of a unit: keys or values, and their scales
 template <int D> struct UnitData<F16, D> {
     uint4_t x[D / 32];
-    __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t at, uint32_t) {
+    template <bool STREAM> __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t at, uint32_t) {
         const uint8_t *p = u + (values ? 32 * D : 0) + at;
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) x[c] = *(const uint4_t *)(p + c * 1024);
+        for (int c = 0; c < D / 32; c++) x[c] = sixteen<STREAM>(p + c * 1024);
     }
     // Of values: zeros in place of the lane's tokens that `keep` (two halves a word) has no bits for; which of the four tokens hold what is not finite (bits of 0x7c00 in each half)
     __device__ __forceinline__ void mask(uint2_t keep) {
@@ -159,10 +161,10 @@ template <int D> struct UnitData<F16, D> {
 };
 template <int D> struct UnitData<Q8, D> {
     uint4_t x[D / 64], s[D / 64];
-    __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t at, uint32_t scale_at) {
+    template <bool STREAM> __device__ __forceinline__ void load(const uint8_t *u, bool values, uint32_t at, uint32_t scale_at) {
         const uint8_t *p = u + (values ? 17 * D : 0);
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) x[c] = *(const uint4_t *)(p + c * 1024 + at);
+        for (int c = 0; c < D / 64; c++) x[c] = sixteen<STREAM>(p + c * 1024 + at);
 #pragma unroll
         for (int c = 0; c < D / 64; c++) s[c] = *(const uint4_t *)(p + 16 * D + scale_at + c * 16);
     }
@@ -363,7 +365,7 @@ struct Part {
 };
 static_assert(sizeof(Part) == QW_ATTN_PART, "");
 
-template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
+template <int TYPE, int D, int QT, bool STREAM> __device__ __forceinline__ void attn_body(const qwk_attn_args &a) {
     constexpr int W = QW_WG_ATTN / 64, U = D <= 128 ? 2 : 1, LD = D + 4, STEPS = 2 / U; // U: units a wave has in hand; a tile is two
     __shared__ float4_t so[W][16 * QT][LD / 4];
     __shared__ float sm[W][16 * QT], sl[W][16 * QT];
@@ -467,9 +469,9 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
         const uint32_t at = lane * 16, scale_at = (lane >> 4) * (D / 4);
         find(key0);
 #pragma unroll
-        for (int k = 0; k < U; k++) A.K[k].load(u[k], false, steps ? at : 0, steps ? scale_at : 0);
+        for (int k = 0; k < U; k++) A.K[k].template load<STREAM>(u[k], false, steps ? at : 0, steps ? scale_at : 0);
 #pragma unroll
-        for (int k = 0; k < U; k++) A.V[k].load(u[k], true, steps ? at : 0, steps ? scale_at : 0);
+        for (int k = 0; k < U; k++) A.V[k].template load<STREAM>(u[k], true, steps ? at : 0, steps ? scale_at : 0);
         // what every query of the block sees: [see_lo, see_hi), and what any of them does: [all_lo, all_hi)
         const int see_hi = s.len - s.n + by(a.by_group, m0) + 1, all_hi = s.len - s.n + by(a.by_group, min(m0 + 16 * QT, M) - 1) + 1;
         const int see_lo = window ? max(0, all_hi - window) : 0, all_lo = window ? max(0, see_hi - window) : 0;
@@ -493,7 +495,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
                 for (int t = 0; t < QT; t++) p[t][k] = A.scores(t, k);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < U; k++) A.K[k].load(u[k], false, nat, nscale);
+            for (int k = 0; k < U; k++) A.K[k].template load<STREAM>(u[k], false, nat, nscale);
             __builtin_amdgcn_sched_barrier(0);
             A.softmax(key, none, edge, p);
             uint32_t odd = 0;
@@ -506,7 +508,7 @@ template <int TYPE, int D, int QT> __device__ __forceinline__ void attn_body(con
                 for (int k = 0; k < U; k++) A.odd_tokens(k, odd >> 16 * k & 0xffff, now[k], key, none, p);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < U; k++) A.V[k].load(u[k], true, nat, nscale);
+            for (int k = 0; k < U; k++) A.V[k].template load<STREAM>(u[k], true, nat, nscale);
         }
         // the waves' results together, in the waves' order
         const bool whole = from == 0 && to == r.cnt;
@@ -618,7 +620,8 @@ template <int QT> __device__ __forceinline__ void join_body(const qwk_attn_args 
 }
 
 #define QW_ATTN(TYPE, D, QT) \
-    extern "C" __global__ __launch_bounds__(QW_WG_ATTN, 2) void qwk_attn_f##TYPE##_d##D##_q##QT(qwk_attn_args a) { attn_body<TYPE, D, QT>(a); }
+    extern "C" __global__ __launch_bounds__(QW_WG_ATTN, 2) void qwk_attn_f##TYPE##_d##D##_q##QT(qwk_attn_args a) { attn_body<TYPE, D, QT, false>(a); } \
+    extern "C" __global__ __launch_bounds__(QW_WG_ATTN, 2) void qwk_attn_f##TYPE##_d##D##_q##QT##_s(qwk_attn_args a) { attn_body<TYPE, D, QT, true>(a); }
 QW_ATTN(1, 64, 1) QW_ATTN(8, 64, 1) QW_ATTN(1, 64, 2) QW_ATTN(8, 64, 2)
 QW_ATTN(1, 128, 1) QW_ATTN(8, 128, 1) QW_ATTN(1, 128, 2) QW_ATTN(8, 128, 2)
 QW_ATTN(1, 192, 1) QW_ATTN(8, 192, 1) QW_ATTN(1, 256, 1) QW_ATTN(8, 256, 1)

@@ -278,6 +278,18 @@ int main(void) {
         const unsigned units = (unsigned)t[i].rows / 16 + 2 * (t[i].rows < 3 ? (unsigned)t[i].rows : 3);
         if (!call(b, READ, &a) || qw_batch_end(b) < 0 || !saw(t[i].type == 1 ? "qwk_kv_read_f1" : "qwk_kv_read_f8", units)) return printf("%zu: %s, %u: %s\n", i, seen[(launches - 1) % 64], seen_gx[(launches - 1) % 64], g->err), 1;
     }
+    // past the caches: one block a slot and 64 MB of pages that the slots may have
+    static qw_buf pool, wide;
+    if (!qw_hip_buf_new_device(g, (size_t)1 << 28, &pool) || !qw_hip_buf_new_device(g, qw_attn_ws_bytes(g, 128), &wide)) return 3;
+    const struct { int rows, pages, max_pages; const char *attn; } past[] = {
+        {3, 8192, 4096, "qwk_attn_f8_d128_q1_s"}, {12, 8192, 4096, "qwk_attn_f8_d128_q2_s"}, {13, 8192, 4096, "qwk_attn_f8_d128_q2"}, {3, 1024, 4096, "qwk_attn_f8_d128_q1"}, {3, 8192, 4, "qwk_attn_f8_d128_q1"}};
+    for (size_t i = 0; i < sizeof past / sizeof *past; i++) {
+        a = right(g);
+        a.c.at.buf = &pool, a.c.heads = 1, a.ws.buf = &wide, a.s.table.buf = &big, a.s.rows = past[i].rows, a.c.pages = past[i].pages, a.s.max_pages = past[i].max_pages;
+        qw_batch *b = qw_batch_begin(g, false);
+        if (!call(b, ATTN, &a) || qw_batch_end(b) < 0 || strcmp(seen[(launches - 2) % 64], past[i].attn)) return printf("past %zu: %s, %s\n", i, seen[(launches - 2) % 64], g->err), 1;
+    }
+    a = right(g);
     qw_batch *b = qw_batch_begin(g, false);
     if (!call(b, SAMPLE, &a) || qw_batch_end(b) < 0 || !saw("qwk_sample", 3)) return printf("%s: %s\n", seen[(launches - 1) % 64], g->err), 1;
     // threads of a workgroup: no other number is recorded
@@ -385,7 +397,7 @@ def test_launches_and_their_workgroups(tmp_path):
     src = subprocess.run([build.HIPCC, "--offload-arch=gfx950", "-std=c++17", "--cuda-device-only", "-E", "-P", "-I", os.path.join(build.CSRC, "kernels"), os.path.join(build.CSRC, "kernels", "qw_attn.hip")],
                          stdout=subprocess.PIPE, text=True, check=True).stdout
     found = re.findall(r"amdgpu_flat_work_group_size\(1,\s*([0-9u* ]+)\)[^;{}]*?void\s+(qwk_\w+)\s*\(", src)
-    assert len(found) == 12 + 2 + 4 + 2 + 2 == len(set(n for _, n in found))
+    assert len(found) == 24 + 2 + 4 + 2 + 2 == len(set(n for _, n in found))
     run(tmp_path, LAUNCHES.replace("@names", ", ".join('{"%s", %s}' % (n, t) for t, n in found)))
 
 

@@ -366,3 +366,16 @@ def test_tokens_beyond_two_to_the_29(gpu, dev, kind):
             assert np.array_equal(got.read(dtype=np.float16).reshape(k.shape)[row], want[0].astype(np.float16))
     want, tol = attention(c, s, qr, 0.125, window)
     assert (np.abs(out.read(dtype=np.float16).reshape(qr.shape) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
+@pytest.mark.parametrize("D,G", [(64, 4), (64, 10), (128, 4), (128, 10), (192, 8), (256, 8)])
+def test_units_past_the_caches(gpu, dev, kind, D, G):
+    """Pages enough for slots of any length that the kernels read past the caches."""
+    rng = np.random.default_rng(D + G)
+    page, H = 64, 1
+    pages = (64 << 20) // (page // 16 * D * (64 if kind == F16 else 34)) + 1
+    s = Step(rng, [1, 2], [700, 95], page, pages=pages)
+    s.table = np.concatenate([s.table, np.full((2, pages), 0xffffffff, np.uint32)], 1)
+    s.max_pages = s.table.shape[1]
+    check(dev, gpu, rng, kind, H, H * G, D, page, s)
