@@ -30,8 +30,8 @@ enum { F16 = 1, Q8 = 8 };
 // Eight waves a workgroup take a share's tiles in turn, each with the next step's units on their way while it works on the last; two workgroups of four a compute unit left twice as much for
 // the join (drafts 32.3 us, not 29.4; one token over 700 tokens 11.9, not 12.1).
 //
-// Bound: by the cache's bytes once there are enough of them. 64 slots of 8192 tokens, binary16, 4 heads of 128 values (1.07 GB) 178 us, 5.9 TB/s; one slot of 131072, Q8_0, 2 heads of 256
-// (143 MB) 30 us and 5 for the join; 16 slots of up to 4096, binary16 (78 MB) 17 and 4. Two blocks of queries make Q8_0 instruction-bound (a step, two units of 128 values, is some
+// Bound: by the cache's bytes once there are enough of them. 64 slots of 8192 tokens, binary16, 4 heads of 128 values (1.07 GB) 160 us, 6.7 TB/s; one slot of 131072, Q8_0, 2 heads of 256
+// (143 MB) 28 us and 5 for the join; 16 slots of up to 4096, binary16 (78 MB) 17 and 4. Two blocks of queries make Q8_0 instruction-bound (a step, two units of 128 values, is some
 // 500 vector and 64 matrix instructions): 12 slots of 45 rows over 6001 tokens 24 us for 55 MB, of which 4 are gone before the first unit arrives. One token over 700: 8.5 us, five
 // dependent round trips to memory and the launch.
 
