@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import qwental_amd as q
-from attn_helpers import F16, Q8, Cache, Step, attention, scale_places, turned
+from attn_helpers import F16, Q8, Cache, Step, attention, scale_places, tolerance, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -379,3 +379,28 @@ def test_units_past_the_caches(gpu, dev, kind, D, G):
     s.table = np.concatenate([s.table, np.full((2, pages), 0xffffffff, np.uint32)], 1)
     s.max_pages = s.table.shape[1]
     check(dev, gpu, rng, kind, H, H * G, D, page, s)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+def test_the_most_rows(gpu, dev, window):
+    """65536 rows of a slot, in, out and attended to; some of them checked."""
+    rng = np.random.default_rng(43)
+    R, page = 65536, 256
+    s = Step(rng, [R], [R], page, spare=0)
+    k, v, qr = rows(rng, R, 1, 64), rows(rng, R, 1, 64), rows(rng, R, 2, 64)
+    kc = q.KvCache(dev.new(q.kv_bytes(gpu.L, F16, 1, 64, page, s.pages)), F16, 1, 64, page, s.pages)
+    st, back, out, ws = dev.step(s), [dev.new(k.nbytes) for _ in range(2)], dev.new(qr.nbytes), dev.new(q.attn_ws_bytes(gpu, 64))
+    qb = dev.up(qr)
+    dev.run(q.KvWrite(kc, st, 2, qb, qb, dev.up(k), dev.up(v)), q.KvRead(kc, st, *back), q.Attn(kc, st, 2, qb, out, ws, window=window))
+    assert np.array_equal(back[0].read(dtype=np.uint16), k.view(np.uint16).ravel()) and np.array_equal(back[1].read(dtype=np.uint16), v.view(np.uint16).ravel())
+    got = out.read(dtype=np.float16).reshape(qr.shape).astype(np.float64)
+    for row in [0, 1, 15, 16, 31, 32, R - 1] + rng.integers(0, R, 60).tolist():
+        a = max(0, row + 1 - window) if window else 0
+        kk, vv = (x[a:row + 1, 0].astype(np.float64) for x in (k, v))
+        x = qr[row].astype(np.float64) @ kk.T / 8
+        size = (np.abs(qr[row].astype(np.float64)) @ np.abs(kk).T / 8).max(1, keepdims=True)
+        p = np.exp(x - x.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        want = p @ vv
+        floor = len(kk) * p.max(1, keepdims=True) * 2.0 ** -39 * np.abs(vv).max()
+        assert (np.abs(got[row] - want) <= tolerance(want, p @ np.abs(vv), size, len(kk), 64) + floor).all(), row
